@@ -268,7 +268,7 @@ def prepare(c, seed):
         s["cache"].import_blocks(torch.arange(blocks, dtype=torch.int32, device="cuda"), kc, vc,
                                  ksc, vsc)
         if c["op"] == "attention":
-            s["space"] = lib.AttentionWorkspace(s["cache"], c["heads"], n, tokens)
+            s["space"] = lib.AttentionWorkspace(s["cache"])
             s["out"] = torch.empty_like(s["q"])
             s["lse"] = torch.empty((tokens, c["heads"]), device="cuda")
     else:
