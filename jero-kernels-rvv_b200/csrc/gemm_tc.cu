@@ -53,6 +53,7 @@
 
 #include "jkb_internal.h"
 #include "nibble.cuh"
+#include "ptx.cuh"
 
 namespace jkb {
 
@@ -61,7 +62,6 @@ namespace {
 constexpr int BMW = 128;  // weight rows per tile (MMA M, TMEM lanes)
 constexpr int BK = 128;   // K bytes per stage
 constexpr int GPS = 4;    // scale groups per stage
-constexpr unsigned long long WAIT_NS = 2000000000ull;  // bounded waits: 2 s
 
 template <int BN_, int WPQ_, int GPR_, bool EXACT_, bool MINS_ = false, bool H16_ = false,
           int NIB_ = NIB_NONE, int AB_ = 1, int CTAS_ = 1>
@@ -169,74 +169,6 @@ struct TcSmem {
 
 // ---------------------------------------------------------------- PTX helpers
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-    return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ unsigned long long globaltimer() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-__device__ __forceinline__ void mbar_init(uint64_t *b, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count));
-}
-__device__ __forceinline__ bool mbar_try(uint64_t *b, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(b)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// Waits for the phase of parity `parity` to complete; false after WAIT_NS or when another role
-// has aborted.
-__device__ __forceinline__ bool mbar_wait_slow(uint64_t *b, uint32_t parity, volatile int *abort_flag,
-                                               int *err) {
-    const unsigned long long t0 = globaltimer();
-    for (uint32_t i = 1;; i++) {
-        if (mbar_try(b, parity)) return true;
-        if ((i & 255) == 0) {
-            if (*abort_flag) return false;
-            if (globaltimer() - t0 > WAIT_NS) {
-                *abort_flag = 1;
-                atomicOr(err, 1);
-                return false;
-            }
-        }
-    }
-}
-__device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity, volatile int *abort_flag,
-                                          int *err) {
-    return mbar_try(b, parity) || mbar_wait_slow(b, parity, abort_flag, err);
-}
-// Bounded like mbar_wait_slow, with a short sleep between polls: for warps that run ahead of
-// the MMA and would otherwise take issue slots from the epilogue warps.
-__device__ __forceinline__ bool mbar_wait_sleepy(uint64_t *b, uint32_t parity,
-                                                 volatile int *abort_flag, int *err) {
-    if (mbar_try(b, parity)) return true;
-    const unsigned long long t0 = globaltimer();
-    for (;;) {
-        __nanosleep(256);
-        if (mbar_try(b, parity)) return true;
-        if (*abort_flag) return false;
-        if (globaltimer() - t0 > WAIT_NS) {
-            *abort_flag = 1;
-            atomicOr(err, 1);
-            return false;
-        }
-    }
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t *b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_tx(uint64_t *b, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)),
-                 "r"(bytes)
-                 : "memory");
-}
 // 2-D TMA tile load (no multicast) completing on mbarrier b.
 __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *tm, uint64_t *b, int x,
                                             int y) {
@@ -245,17 +177,6 @@ __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *tm, ui
         " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
         "l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(b)), "r"(x), "r"(y)
         : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() {
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_commit(uint64_t *b) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                     smem_u32(b))
-                 : "memory");
 }
 // D[tmem] = A[smem desc] x B[smem desc]^T, int8 x int8 -> int32 (D is overwritten)
 __device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
@@ -289,47 +210,10 @@ __device__ __forceinline__ void tmem_ld16x256(uint32_t taddr, uint32_t (&r)[16])
           "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld_wait() {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-// K-major operand tile of 128-byte rows with the 128-byte swizzle: 8-row atoms 1024 bytes apart.
-__device__ __forceinline__ uint64_t smem_desc(const void *p) {
-    const uint64_t addr = smem_u32(p);
-    return ((addr >> 4) & 0x3FFFull)           // start address
-           | (1ull << 16)                      // leading byte offset (unused with swizzle)
-           | ((uint64_t)(1024 >> 4) << 32)     // stride byte offset: next 8-row atom
-           | (1ull << 46)                      // descriptor version (sm_100)
-           | (2ull << 61);                     // SWIZZLE_128B
-}
 // kind::i8 instruction descriptor: D s32, A s8, B s8, both K-major, M = 128, N = bn.
 __host__ __device__ constexpr uint32_t idesc_i8(int bn) {
     return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(bn >> 3) << 17) |
            ((uint32_t)(BMW >> 4) << 24);
-}
-
-// Packed f32 pairs (two outputs per instruction).
-__device__ __forceinline__ uint64_t pk2(uint32_t lo, uint32_t hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
-__device__ __forceinline__ void upk2(uint64_t v, float &lo, float &hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
 }
 
 // Distributed shared memory of a thread-block cluster: the address of this CTA's shared
