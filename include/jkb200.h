@@ -116,8 +116,11 @@ int jkb_last_error_info(jkb_error_info *out);
 void jkb_clear_error(void);
 /* No reference counterpart: the device error word of the kernels with bounded waits (bit 0: a
  * wait in the tensor-core GEMM expired, so that call's output is not valid; bit 1: a peer-group
- * wait expired). Synchronizes `stream`, copies the word to *flags, clears it, and returns
- * JKB_E_TIMEOUT when it was non-zero, JKB_OK otherwise. */
+ * wait expired; bit 3: a wait in attention expired) and of the key/value cache's kernels, which
+ * find block ids, slots and lengths only on the device (bit 2: one was out of range; what it
+ * names was neither read nor written). Synchronizes `stream`, copies the word to *flags, clears
+ * it, and returns JKB_E_TIMEOUT when a wait expired, JKB_E_BOUNDS when bit 2 alone was set, JKB_OK
+ * when the word was 0. */
 int jkb_device_status(int32_t *flags, void *stream);
 /* No reference counterpart: the f32 epilogue of the tensor-core repacked GEMM (scale groups
  * of 32 or 16 elements, batches of at least 16 tokens; Q2_K from 32). 0 (the default): acc = fma((f32)c, xs * ws, acc)
@@ -698,6 +701,112 @@ int jkb_peer_group_wait(jkb_peer_group *pg, uint64_t arrivals, void *stream);
 int jkb_peer_group_set_push(jkb_peer_group *pg, int enable);
 int jkb_peer_group_signal(jkb_peer_group *pg, void *stream);
 int jkb_peer_group_destroy(jkb_peer_group *pg);
+
+/* ---- key/value cache in 8 bits, and attention over it (no reference counterpart) ----
+ * What a decoder layer needs between its q/k/v projections and its output projection: a paged
+ * cache of int8 keys and values with one f32 scale per (block of tokens, kv head) for the keys
+ * and one for the values, block tables and slot maps built on the device from request lengths,
+ * and softmax(scale * q k^T) v over the cached tokens.
+ *
+ * A cache holds n_blocks blocks of block_tokens (16, 32, 64 or 128) tokens for n_kv_heads heads
+ * of head_dim (a multiple of 8, at most 256) elements; n_blocks * block_tokens <= 2^31 - 1. The
+ * token of slot s is token s % block_tokens of block s / block_tokens. A value is code * scale,
+ * |code| <= 127. Codes lie in the order in which the attention kernels' matrix instructions take
+ * them (jkb_kv_cache_import and _export convert). Block ids, slots, lengths and starts are read
+ * on the device; ids and slots that are out of range are skipped and reported by
+ * jkb_device_status (bit 2). A sequence's lengths are clamped to its table row. */
+typedef struct jkb_kv_cache jkb_kv_cache;
+/* Allocates the codes (2 * n_blocks * n_kv_heads * block_tokens bytes per element of head_dim,
+ * that rounded up to 64, 96, 128, 192 or 256) and scales, all zero. */
+int jkb_kv_cache_create(size_t n_blocks, size_t block_tokens, size_t n_kv_heads, size_t head_dim,
+                        jkb_kv_cache **out);
+int jkb_kv_cache_destroy(jkb_kv_cache *cache);
+int jkb_kv_cache_info(const jkb_kv_cache *cache, size_t *n_blocks, size_t *block_tokens,
+                      size_t *n_kv_heads, size_t *head_dim, size_t *device_bytes);
+/* Copies blocks in and out: `blocks` are n distinct block ids (device); codes are
+ * [n][n_kv_heads][block_tokens][head_dim] int8, scales [n][n_kv_heads] f32 (device). */
+int jkb_kv_cache_import(jkb_kv_cache *cache, const int32_t *blocks, size_t n,
+                        const int8_t *k_codes, const int8_t *v_codes, const float *k_scales,
+                        const float *v_scales, void *stream);
+int jkb_kv_cache_export(const jkb_kv_cache *cache, const int32_t *blocks, size_t n,
+                        int8_t *k_codes, int8_t *v_codes, float *k_scales, float *v_scales,
+                        void *stream);
+/* The values code * scale of n blocks, [n][n_kv_heads][block_tokens][head_dim] f32 each. */
+int jkb_kv_cache_read(const jkb_kv_cache *cache, const int32_t *blocks, size_t n, float *k_out,
+                      float *v_out, void *stream);
+
+/* Rows of one tensor: element e of head h of token t is data[t * token_stride + h * head_stride
+ * + e] (strides in elements; a part of a fused projection's output is one). `type` is JKB_F32,
+ * JKB_F16 or JKB_BF16. */
+typedef struct {
+    const void *data;
+    int32_t type;
+    size_t token_stride;
+    size_t head_stride;
+} jkb_rows;
+/* Writes the key and value rows of n_tokens tokens to their slots (device; a negative slot skips
+ * its token). Per block, head and side the scale is absmax * f32(1 / 127): a block whose first
+ * new token has offset 0 starts with the new rows' alone; otherwise it keeps the larger of its
+ * own and theirs, and where it grew the earlier codes of the block (offsets below the first new
+ * one) become rint(code * (old / new)). New codes are rint(x * (1 / scale)), ties to even;
+ * non-finite elements count as 0, a scale below the smallest normal f32 is 0. The tokens of one
+ * block must stand together in the call, in consecutive slots; one that leaves a gap is skipped
+ * and reported (bit 2). */
+int jkb_kv_append(jkb_kv_cache *cache, const jkb_rows *k, const jkb_rows *v,
+                  const int32_t *slots, size_t n_tokens, void *stream);
+
+/* Builds a step's block tables and slot map on the device (n_seqs <= JKB_KV_MAX_SEQS). Sequence
+ * i holds ctx_lens[i] tokens and adds new_lens[i]; its row of block_table (row_blocks entries,
+ * rows table_stride apart) already holds the blocks of its ctx_lens[i] tokens. The sequences, in
+ * order, take the whole blocks they need from free_blocks, in order, into their rows. One whose
+ * tokens exceed its row takes none; neither does one for which the list has not enough left, nor
+ * any later one that needs a block. Outputs, all device int32: q_starts [n_seqs + 1], the
+ * exclusive sums of new_lens; slots and positions [n_slots], for the new tokens of all sequences
+ * in order (-1 for the tokens of a sequence that found no room, and from the last token on);
+ * kv_lens [n_seqs], ctx + new (ctx where there was no room); counts [3]: new tokens, blocks
+ * taken, sequences without room. Negative lengths count as 0. New tokens past n_slots get no
+ * slot (counts[0] says how many there are). */
+#define JKB_KV_MAX_SEQS 8192
+int jkb_kv_build_tables(int32_t *block_table, size_t n_seqs, size_t row_blocks,
+                        size_t table_stride, int32_t *slots, int32_t *positions, size_t n_slots,
+                        int32_t *q_starts, int32_t *kv_lens, int32_t *counts,
+                        const int32_t *ctx_lens, const int32_t *new_lens,
+                        const int32_t *free_blocks, size_t n_free, size_t block_tokens,
+                        void *stream);
+
+/* Scratch of the attention calls over caches of one head_dim: partial results where the tokens
+ * of a sequence are split over the GPU. Calls that may overlap on the GPU need one each. */
+typedef struct jkb_attn_workspace jkb_attn_workspace;
+int jkb_attn_workspace_create(const jkb_kv_cache *cache, jkb_attn_workspace **out);
+int jkb_attn_workspace_destroy(jkb_attn_workspace *ws);
+
+/* Attention of the query tokens q_starts[i] .. q_starts[i + 1] of each sequence i over its
+ * kv_lens[i] cached tokens (its last ones being the query tokens themselves: query token r of n
+ * stands at position p = kv_lens[i] - n + r). It sees the tokens j < kv_lens[i] with j <= p
+ * (causal) and j > p - window (window > 0):
+ *   out[t][h] = sum_j w_j v_j,  w_j = exp(s_j) / sum exp(s),  s_j = scale * q[t][h] . k_j,
+ * keys and values of kv head h / (n_heads / n_kv_heads); lse[t][h] = log sum_j exp(s_j). A query
+ * that sees no token has out = 0 and lse = -inf; one with a non-finite element has NaN.
+ * q and out share a type; out rows may be strided too. Sums, softmax statistics and the
+ * accumulated output are f32 for every type. max_new: an upper bound of the query tokens of a
+ * sequence (it selects the kernels; outputs stay right above it, but slow). */
+typedef struct {
+    const jkb_kv_cache *cache;
+    jkb_attn_workspace *ws;
+    jkb_rows q;
+    jkb_rows out;               /* data is written */
+    float *lse;                 /* [n_tokens][n_heads] or NULL */
+    size_t n_tokens, n_heads;
+    const int32_t *block_table; /* [n_seqs] rows of row_blocks ids, table_stride apart */
+    const int32_t *kv_lens;     /* [n_seqs] */
+    const int32_t *q_starts;    /* [n_seqs + 1] */
+    size_t n_seqs, row_blocks, table_stride;
+    size_t max_new;
+    size_t window;              /* 0: none */
+    float scale;
+    int32_t causal;
+} jkb_attn_args;
+int jkb_attention_kv8(const jkb_attn_args *args, void *stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

@@ -3,6 +3,7 @@
 #include <cstring>
 
 #include "jkb_internal.h"
+#include "kv_cache.cuh"
 
 namespace jkb {
 
@@ -160,8 +161,9 @@ int validate_weight_call(const char *fn, const jkb_weight *w, int expected_quant
 }
 
 // Device error word shared by the kernels with bounded waits: bit 0, a wait in the tensor-core
-// GEMM expired; bit 1, a peer-group wait (peer.cu) expired. Kernels get its address as an
-// argument; host code reads and clears it in jkb_device_status.
+// GEMM expired; bit 1, a peer-group wait (peer.cu) expired; ERR_KV_RANGE and ERR_ATTN_WAIT, see
+// kv_cache.cuh. Kernels get its address as an argument; host code reads and clears it in
+// jkb_device_status.
 __device__ int g_device_error;
 
 int *device_error_word() {
@@ -195,9 +197,14 @@ int jkb_device_status(int32_t *flags, void *stream) {
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
     if (e != cudaSuccess) return fail_cuda(e, "device_status");
     *flags = v;
-    return v ? fail(JKB_E_TIMEOUT, "device_status", 0, 0, 0,
+    if (v & ~ERR_KV_RANGE)
+        return fail(JKB_E_TIMEOUT, "device_status", 0, 0, 0,
                     "a bounded wait expired on the device (flags %d: bit 0 tensor-core GEMM, "
-                    "bit 1 peer-group wait)",
+                    "bit 1 peer-group wait, bit 3 attention)",
+                    v);
+    return v ? fail(JKB_E_BOUNDS, "device_status", 0, 0, 0,
+                    "a block id, slot or length of the key/value cache was out of range on the "
+                    "device (flags %d)",
                     v)
              : JKB_OK;
 }

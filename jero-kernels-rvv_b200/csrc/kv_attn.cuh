@@ -1,0 +1,53 @@
+// What the two attention kernels share (kv_attn.cu: few query rows; kv_attn_tc.cu: prompts).
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace jkb {
+
+struct AttnParams {
+    const uint8_t *codes;
+    const float2 *scales;
+    int n_blocks, kv_heads, log_block, dim;
+    int group;  // query heads of a kv head
+    const void *q;
+    void *out;
+    size_t q_token, q_head, out_token, out_head;
+    int q_vec, out_vec;  // rows may be read / written 16 bytes at a time
+    float *lse;
+    int n_tokens;
+    const int32_t *table, *kv_lens, *q_starts;
+    size_t table_stride;
+    int n_seqs, row_blocks;
+    int window, causal;
+    float scale2;        // scale * log2(e): the softmax works in powers of two
+    int min_rows, max_rows;  // query rows (tokens * group) of the sequences this launch takes
+    float *partial;
+    int *counters;
+    int *err;
+};
+
+// One sequence of a launch: query tokens q0 .. q0 + nq, cached tokens len, the visible ones
+// lo .. len. nq = 0 where the launch does not take it.
+struct AttnSeq {
+    int q0, nq, len, lo;
+};
+__device__ __forceinline__ AttnSeq attn_seq(const AttnParams &p, int i) {
+    AttnSeq s;
+    s.q0 = min(max(__ldg(p.q_starts + i), 0), p.n_tokens);
+    const int q1 = min(max(__ldg(p.q_starts + i + 1), s.q0), p.n_tokens);
+    s.nq = q1 - s.q0;
+    const long long rows = (long long)s.nq * p.group;
+    if (rows < p.min_rows || rows > p.max_rows) s.nq = 0;
+    const int room = p.row_blocks << p.log_block, len = __ldg(p.kv_lens + i);
+    if (s.nq && (len < 0 || len > room)) atomicOr(p.err, ERR_KV_RANGE);
+    s.len = min(max(len, 0), room);
+    s.lo = 0;
+    if (p.window) s.lo = min(max((long long)s.len - s.nq + 1 - p.window, 0ll), (long long)s.len);
+    return s;
+}
+
+int attn_decode_launch(const AttnParams &p, int type, int dim_p, size_t max_rows,
+                       cudaStream_t st);
+
+}  // namespace jkb

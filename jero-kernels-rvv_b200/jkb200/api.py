@@ -42,6 +42,7 @@ __all__ = [
     "gemv_repacked_view_rows", "gemv_repacked_f32", "gemv_repacked_f32_rows",
     "gemm_repacked_f32_rows", "BlockScaledTileLayout", "block_scaled_layout",
     "repack_into_tile_range", "repack_q4_k_m_parallel_slices",
+    "KvCache", "kv_append", "kv_build_tables", "AttentionWorkspace", "attention_kv8",
 ]
 
 
@@ -132,8 +133,9 @@ def abi_version() -> int:
 
 
 def device_status(stream=None) -> int:
-    """Synchronizes the stream and returns (and clears) the device error word of the
-    tensor-core GEMM; raises K3Error (JKB_E_TIMEOUT) when a bounded wait in it expired."""
+    """Synchronizes the stream and returns (and clears) the device error word; raises K3Error
+    (JKB_E_TIMEOUT) when a bounded wait in a kernel expired, TensorBoundsError when a block id,
+    slot or length of the key/value cache was out of range on the device."""
     v = C.c_int32(0)
     _check(_L().jkb_device_status(C.byref(v), _stream(stream)))
     return int(v.value)
@@ -1297,3 +1299,200 @@ def repack_q4_k_m_parallel_slices(view: TensorView, rows: int, cols: int, tile_r
         C.byref(v), rows, cols, tile_range.start, tile_range.stop, out_tiles_i8.ctypes.data,
         out_tiles_i8.size, out_scales.ctypes.data, out_scales.size, out_mins.ctypes.data,
         out_mins.size))
+
+
+# ------------------------------------------------------------------------------- 8-bit kv cache
+
+_ROW_TYPES = {torch.float32: int(QuantType.F32), torch.float16: int(QuantType.F16),
+              torch.bfloat16: int(QuantType.BF16)}
+
+
+def _rows(t: torch.Tensor, what: str, heads: int = None, dim: int = None) -> "_lib.jkb_rows":
+    """jkb_rows of a [tokens, heads, dim] CUDA tensor whose elements of a head are adjacent."""
+    if not t.is_cuda or t.dim() != 3:
+        raise TypeError(f"{what}: expected a [tokens, heads, dim] CUDA tensor")
+    kind = _ROW_TYPES.get(t.dtype)
+    if kind is None:
+        raise TypeError(f"{what}: {t.dtype} is none of float32, float16 and bfloat16")
+    shape, stride = t.shape, t.stride()
+    if (heads is not None and shape[1] != heads) or (dim is not None and shape[2] != dim):
+        raise ValueError(f"{what}: shape {tuple(shape)}, expected [tokens, {heads}, {dim}]")
+    if stride[2] != 1 and shape[2] > 1 or stride[0] < 0 or stride[1] < 0:
+        raise ValueError(f"{what}: the elements of a head must be adjacent")
+    return _lib.jkb_rows(t.data_ptr(), kind, stride[0], stride[1])
+
+
+def _i32(t: torch.Tensor, what: str) -> int:
+    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+        raise TypeError(f"{what}: expected a contiguous int32 CUDA tensor")
+    return t.data_ptr()
+
+
+def _table(t: torch.Tensor):
+    """(pointer, rows, blocks a row, row stride) of a [sequences, blocks] int32 table."""
+    if t.dtype != torch.int32 or not t.is_cuda or t.dim() != 2:
+        raise TypeError("block_table: expected a [sequences, blocks] int32 CUDA tensor")
+    n, width = t.shape
+    s0, s1 = t.stride()
+    if s1 != 1 and width > 1 or (n > 1 and s0 < width):
+        raise ValueError("block_table: the ids of a row must be adjacent")
+    return t.data_ptr(), n, width, max(s0, width)
+
+
+class KvCache:
+    """A paged key/value cache of int8 codes with one f32 scale for the keys and one for the
+    values of each block of tokens and kv head (no reference counterpart). The token of slot s is
+    token s % block_tokens of block s // block_tokens; block_tokens is 16, 32, 64 or 128 and
+    head_dim a multiple of 8 up to 256. Fresh blocks hold zeros."""
+
+    def __init__(self, n_blocks: int, block_tokens: int, n_kv_heads: int, head_dim: int):
+        h = C.c_void_p()
+        _check(_L().jkb_kv_cache_create(n_blocks, block_tokens, n_kv_heads, head_dim,
+                                        C.byref(h)))
+        self._h = h.value
+        self.n_blocks, self.block_tokens = n_blocks, block_tokens
+        self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
+        n = C.c_size_t()
+        _check(_L().jkb_kv_cache_info(self._h, None, None, None, None, C.byref(n)))
+        self.device_bytes = n.value
+
+    @property
+    def handle(self):
+        if self._h is None:
+            raise InvalidHandle(6, "kv_cache", 0, 0, 0, "kv cache destroyed")
+        return self._h
+
+    def _planes(self, blocks, k, v, dtype):
+        n = blocks.numel()
+        shape = (n, self.n_kv_heads, self.block_tokens, self.head_dim)
+        for t in (k, v):
+            if t.dtype != dtype or tuple(t.shape) != shape:
+                raise ValueError(f"expected {dtype} planes of shape {shape}, got {t.dtype} "
+                                 f"{tuple(t.shape)}")
+        return _i32(blocks, "blocks"), n, _dptr(k), _dptr(v)
+
+    def _scales(self, blocks, k, v):
+        for t in (k, v):
+            if t.dtype != torch.float32 or tuple(t.shape) != (blocks.numel(), self.n_kv_heads):
+                raise ValueError(f"expected float32 scales of shape "
+                                 f"{(blocks.numel(), self.n_kv_heads)}")
+        return _dptr(k), _dptr(v)
+
+    def import_blocks(self, blocks, k_codes, v_codes, k_scales, v_scales, stream=None):
+        """Sets the blocks (distinct int32 ids): codes int8 [n, kv heads, block tokens, head dim],
+        scales float32 [n, kv heads]."""
+        a = self._planes(blocks, k_codes, v_codes, torch.int8)
+        _check(_L().jkb_kv_cache_import(self.handle, *a, *self._scales(blocks, k_scales, v_scales),
+                                        _stream(stream)))
+
+    def export_blocks(self, blocks, k_codes, v_codes, k_scales, v_scales, stream=None):
+        """Copies the blocks' codes and scales out, in the layout of import_blocks."""
+        a = self._planes(blocks, k_codes, v_codes, torch.int8)
+        _check(_L().jkb_kv_cache_export(self.handle, *a, *self._scales(blocks, k_scales, v_scales),
+                                        _stream(stream)))
+
+    def read_blocks(self, blocks, k_out, v_out, stream=None):
+        """The values code * scale of the blocks, float32 [n, kv heads, block tokens, head dim]."""
+        _check(_L().jkb_kv_cache_read(self.handle, *self._planes(blocks, k_out, v_out,
+                                                                 torch.float32),
+                                      _stream(stream)))
+
+    def destroy(self):
+        if getattr(self, "_h", None):
+            _L().jkb_kv_cache_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
+def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, stream=None):
+    """Quantizes the key and value rows [tokens, kv heads, head dim] (float32, float16 or
+    bfloat16; parts of a fused projection may be strided) into their slots (int32; negative:
+    skipped). The tokens of a block stand together, in consecutive slots. A block's scale is its
+    absmax / 127: fresh where its first new token has offset 0, else the larger of its own and the
+    new rows', its earlier codes being rounded again where it grew."""
+    kr = _rows(k, "k", cache.n_kv_heads, cache.head_dim)
+    vr = _rows(v, "v", cache.n_kv_heads, cache.head_dim)
+    n = slots.numel()
+    if k.shape[0] != n or v.shape[0] != n:
+        raise ValueError(f"{k.shape[0]} key rows and {v.shape[0]} value rows for {n} slots")
+    _check(_L().jkb_kv_append(cache.handle, kr, vr, _i32(slots, "slots"), n, _stream(stream)))
+
+
+def kv_build_tables(block_table, slots, positions, q_starts, kv_lens, counts, ctx_lens, new_lens,
+                    free_blocks, block_tokens: int, stream=None):
+    """Builds a step's block tables and slot map on the GPU, all int32 tensors: sequence i holds
+    ctx_lens[i] tokens, whose blocks its row of block_table [sequences, blocks] has, and adds
+    new_lens[i]; the blocks it needs come from free_blocks, in order. Writes the rows' new
+    entries, slots and positions of the new tokens (-1 where there was no room, and past the last
+    token), q_starts [sequences + 1], kv_lens [sequences] and counts [3]: new tokens, blocks
+    taken, sequences without room."""
+    ptr, n, width, stride = _table(block_table)
+    if (ctx_lens.numel() != n or new_lens.numel() != n or kv_lens.numel() != n
+            or q_starts.numel() != n + 1 or counts.numel() != 3
+            or positions.numel() != slots.numel()):
+        raise ValueError("lengths of the tables' tensors do not match")
+    _check(_L().jkb_kv_build_tables(
+        ptr, n, width, stride, _i32(slots, "slots"), _i32(positions, "positions"), slots.numel(),
+        _i32(q_starts, "q_starts"), _i32(kv_lens, "kv_lens"), _i32(counts, "counts"),
+        _i32(ctx_lens, "ctx_lens"), _i32(new_lens, "new_lens"), _i32(free_blocks, "free_blocks"),
+        free_blocks.numel(), block_tokens, _stream(stream)))
+
+
+class AttentionWorkspace:
+    """Scratch of attention_kv8 over caches of this head_dim; calls that may overlap on the GPU
+    need one each."""
+
+    def __init__(self, cache: KvCache):
+        h = C.c_void_p()
+        _check(_L().jkb_attn_workspace_create(cache.handle, C.byref(h)))
+        self._h = h.value
+
+    @property
+    def handle(self):
+        if self._h is None:
+            raise InvalidHandle(6, "attn_workspace", 0, 0, 0, "attention workspace destroyed")
+        return self._h
+
+    def destroy(self):
+        if getattr(self, "_h", None):
+            _L().jkb_attn_workspace_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
+def attention_kv8(out, q, cache: KvCache, workspace: AttentionWorkspace, block_table, kv_lens,
+                  q_starts, max_new: int, scale: float, causal: bool = True, window: int = 0,
+                  lse=None, stream=None):
+    """softmax(scale * q k^T) v over the cached tokens: query tokens q_starts[i] .. q_starts[i+1]
+    of sequence i are its last ones among kv_lens[i] (write them with kv_append first). q and out
+    are [tokens, heads, head dim] of one type, float32, float16 or bfloat16; query head h reads kv
+    head h // (heads / kv heads). window > 0 hides tokens that are window or more back. A query
+    that sees nothing gives 0 and lse -inf. lse: None or float32 [tokens, heads]."""
+    n, heads = q.shape[0], q.shape[1]
+    qr = _rows(q, "q", heads, cache.head_dim)
+    outr = _rows(out, "out", heads, cache.head_dim)
+    if out.shape[0] != n:
+        raise ValueError(f"{out.shape[0]} output rows for {n} queries")
+    if window < 0 or max_new < 0:
+        raise ValueError("window and max_new cannot be negative")
+    if lse is not None and (lse.dtype != torch.float32 or lse.numel() != n * heads):
+        raise ValueError(f"lse: expected float32 [{n}, {heads}]")
+    ptr, seqs, width, stride = _table(block_table)
+    if kv_lens.numel() != seqs or q_starts.numel() != seqs + 1:
+        raise ValueError(f"{kv_lens.numel()} lengths and {q_starts.numel()} starts for {seqs} "
+                         "sequences")
+    args = _lib.jkb_attn_args(
+        cache.handle, workspace.handle, qr, outr, _dptr(lse), n, heads, ptr,
+        _i32(kv_lens, "kv_lens"), _i32(q_starts, "q_starts"), seqs, width, stride, max_new,
+        window, scale, 1 if causal else 0)
+    _check(_L().jkb_attention_kv8(args, _stream(stream)))
