@@ -475,8 +475,8 @@ __global__ void __launch_bounds__(32 * NW, C::CTAS)
             // ---- o = o * alpha + p v ----
 #pragma unroll
             for (int c = 0; c < DT; c++) {
-                const uint4 v4 = *reinterpret_cast<const uint4 *>(stage + 16 * DIM + c * 512 +
-                                                                  lane * 16);
+                const uint4 v4 = *reinterpret_cast<const uint4 *>(
+                    stage + 16 * DIM + c * 512 + (tg * 8 + (g ^ (2 * tg))) * 16);
                 const uint32_t vw[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
@@ -697,15 +697,19 @@ int jkb_attn_workspace_create(const jkb_kv_cache *cache, jkb_attn_workspace **ou
     w->device = cache->device;
     w->dim_p = cache->dim_p;
     w->ctas = 3 * num_sms();
-    const size_t part = (size_t)2 * w->ctas * ATTN_ROWS * (w->dim_p + 2) * sizeof(float);
-    uint8_t *base = nullptr;
-    cudaError_t e = cudaMalloc(&base, Arena::round(part) + w->ctas * sizeof(int));
+    const size_t sms = (size_t)num_sms(), width = (size_t)w->dim_p + 2;
+    const size_t part = Arena::round(2 * (size_t)w->ctas * ATTN_ROWS * width * sizeof(float));
+    const size_t tile = w->dim_p <= 128 ? Arena::round(2 * sms * 128 * width * sizeof(float)) : 0;
+    const size_t counts = (w->ctas + sms) * sizeof(int);
+    cudaError_t e = cudaMalloc(&w->base, part + tile + counts);
     if (e == cudaSuccess) {
-        w->partial = (float *)base;
-        w->counters = (int *)(base + Arena::round(part));
-        e = cudaMemset(w->counters, 0, w->ctas * sizeof(int));
+        w->partial = (float *)w->base;
+        w->tile_partial = tile ? (float *)(w->base + part) : nullptr;
+        w->counters = (int *)(w->base + part + tile);
+        w->tile_counters = w->counters + w->ctas;
+        e = cudaMemset(w->counters, 0, counts);
         if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
-        if (e != cudaSuccess) cudaFree(base);
+        if (e != cudaSuccess) cudaFree(w->base);
     }
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -723,7 +727,7 @@ int jkb_attn_workspace_destroy(jkb_attn_workspace *w) {
         return fail(JKB_E_INVALID, "attn_workspace", 0, 0, 0,
                     "null or destroyed attention workspace handle");
     w->magic = 0;
-    cudaFree(w->partial);
+    cudaFree(w->base);
     free(w);
     return JKB_OK;
 }
@@ -804,9 +808,21 @@ int jkb_attention_kv8(const jkb_attn_args *a, void *stream) {
     p.max_rows = INT32_MAX;
     p.partial = w->partial;
     p.counters = w->counters;
+    p.tile_partial = w->tile_partial;
+    p.tile_counters = w->tile_counters;
     p.err = device_error_word();
     if (!p.err) return fail(JKB_E_CUDA, fn, 0, 0, 0, "no device error word");
-    return attn_decode_launch(p, type, c->dim_p, a->max_new * p.group, as_stream(stream));
+    cudaStream_t st = as_stream(stream);
+    // Sequences of up to ATTN_ROWS query rows a kv head go to the few-row kernel, the others to
+    // the prompt kernel; each leaves the other's alone. max_new tells which of them a call needs.
+    const size_t most = a->max_new * p.group;
+    if (most <= ATTN_ROWS || c->dim_p > 128)
+        return attn_decode_launch(p, type, c->dim_p, most, st);
+    p.max_rows = ATTN_ROWS;
+    if (a->n_seqs > 1 && (rc = attn_decode_launch(p, type, c->dim_p, ATTN_ROWS, st))) return rc;
+    p.min_rows = a->n_seqs > 1 ? ATTN_ROWS + 1 : 1;
+    p.max_rows = INT32_MAX;
+    return attn_prompt_launch(p, type, c->dim_p, st);
 }
 
 }  // extern "C"

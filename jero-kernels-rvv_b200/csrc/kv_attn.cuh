@@ -22,8 +22,10 @@ struct AttnParams {
     int window, causal;
     float scale2;        // scale * log2(e): the softmax works in powers of two
     int min_rows, max_rows;  // query rows (tokens * group) of the sequences this launch takes
-    float *partial;
+    float *partial;       // the workspace's (kv_cache.cuh)
     int *counters;
+    float *tile_partial;
+    int *tile_counters;
     int *err;
 };
 
@@ -49,5 +51,8 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnParams &p, int i) {
 
 int attn_decode_launch(const AttnParams &p, int type, int dim_p, size_t max_rows,
                        cudaStream_t st);
+
+// Sequences of at most `rows` query rows a kv head are few-row ones; head sizes up to 128.
+int attn_prompt_launch(const AttnParams &p, int type, int dim_p, cudaStream_t st);
 
 }  // namespace jkb

@@ -288,7 +288,8 @@ __device__ __forceinline__ void append_run(const Run &r, const AppendSide &src, 
             }
             *at = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
-            const int chunk = p >> 5, q = p & 31, d0 = 32 * chunk + 4 * (q >> 2), t = q & 3;
+            const int chunk = p >> 5, q = p & 31, t = q >> 3;
+            const int d0 = 32 * chunk + 4 * ((q & 7) ^ (2 * t));
             uint4 *at = reinterpret_cast<uint4 *>(g + 16 * dim_p + 512 * chunk + 16 * q);
             bool is_new[4], is_old[4], any = false, keep = false;
 #pragma unroll
@@ -444,7 +445,8 @@ __global__ void __launch_bounds__(COPY_THREADS)
         // (token, dim) of the patch's byte `b`: keys token kt, dims kd ..; values 4 x 4
         const int kc = q >> 4, kt = 8 * (q / (dim_p >> 1)) + ((q % (dim_p >> 1)) & 15) / 2;
         const int kd = 32 * (kc % (dim_p >> 5)) + 16 * (q & 1);
-        const int vd = 32 * (q >> 5) + 4 * ((q & 31) >> 2), vt = 2 * (q & 3);
+        const int vrow = (q >> 3) & 3, vt = 2 * vrow;
+        const int vd = 32 * (q >> 5) + 4 * ((q & 7) ^ vt);
         uint32_t w[4] = {0, 0, 0, 0};
         if (MODE != COPY_IMPORT) {
             const uint4 x = *at;

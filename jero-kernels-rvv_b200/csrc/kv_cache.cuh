@@ -7,11 +7,12 @@
 //   keys   [2][dim_p / 32][8 tokens][32 dims]: eight tokens' 32 dims are 256 bytes, of which lane
 //          4 g + t of a warp takes bytes 8 t .. 8 t + 8 of token g -- the B operand of
 //          mma.m16n8k32 with dims in the order 8 t + {0..3}, 8 t + {4..7}. Codes are int8.
-//   values [dim_p / 32][8 (g)][4 (t)][4 (j)][4 tokens]: lane 4 g + t takes 16 bytes: dims 4 g + j
-//          of the 32, tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 -- the B operands of four
-//          mma.m16n8k16 over 16 tokens. Bytes are code + 128, which two byte permutes and a
-//          packed subtraction turn into f16.
-// Both reads are contiguous 256- and 512-byte runs of a warp: free of bank conflicts.
+//   values [dim_p / 32][4 (t)][8][4 (j)][4 tokens]: 16-byte piece (g, t) stands at g ^ 2t of row t
+//          and holds dims 4 g + j of the 32, tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9. Lane 4 g + t
+//          takes piece (g, t), the B operands of four mma.m16n8k16 over 16 tokens; a converter
+//          thread takes pieces (g, 0..3), the 16 tokens of four dims. Bytes are code + 128, which
+//          two byte permutes and a packed subtraction turn into f16.
+// Each of these reads is free of bank conflicts (hence the exclusive or).
 #pragma once
 
 #include "jkb_internal.h"
@@ -25,15 +26,18 @@ struct jkb_kv_cache {
     float2 *scales;  // [n_blocks][n_heads]: (key scale, value scale)
 };
 
-// Partial results of attention pieces, and the counters by which a piece knows that it is its
-// row tile's last (zero between calls).
+// Partial results of attention pieces (two slots a CTA), and the counters by which a piece knows
+// that it is its row tile's last to finish (zero between calls).
 struct jkb_attn_workspace {
     uint32_t magic;
     int device;
     int dim_p;
-    int ctas;          // pieces' slots: 2 per CTA
-    float *partial;    // [2 * ctas][ATTN_ROWS][dim_p + 2]
-    int *counters;     // [ctas]
+    int ctas;             // most CTAs of the few-row kernel; the prompt kernel has one an SM
+    uint8_t *base;
+    float *partial;       // [2 * ctas][ATTN_ROWS][dim_p + 2]
+    float *tile_partial;  // [2 * SMs][dim_p + 2][128]; nullptr above 128 dims
+    int *counters;        // [ctas]
+    int *tile_counters;   // [SMs]
 };
 
 namespace jkb {
@@ -47,14 +51,8 @@ constexpr int ATTN_ROWS = 16;  // most query rows of a decode row tile
 
 int check_kv_cache(const jkb_kv_cache *c, const char *fn);
 
-// Byte of the key code of (token, dim) in its group, and of the value code.
+// Byte of the key code of (token, dim) in its group.
 __host__ __device__ inline int kv_key_at(int token, int dim, int dim_p) {
     return (token >> 3) * 8 * dim_p + (dim >> 5) * 256 + (token & 7) * 32 + (dim & 31);
 }
-__host__ __device__ inline int kv_value_at(int token, int dim, int dim_p) {
-    const int d = dim & 31;
-    return 16 * dim_p + (dim >> 5) * 512 + ((d >> 2) * 4 + ((token & 7) >> 1)) * 16 +
-           (d & 3) * 4 + (token & 1) + 2 * (token >> 3);
-}
-
 }  // namespace jkb

@@ -1334,7 +1334,7 @@ def _table(t: torch.Tensor):
         raise TypeError("block_table: expected a [sequences, blocks] int32 CUDA tensor")
     n, width = t.shape
     s0, s1 = t.stride()
-    if s1 != 1 and width > 1 or (n > 1 and s0 < width):
+    if n and (s1 != 1 and width > 1 or (n > 1 and s0 < width)):
         raise ValueError("block_table: the ids of a row must be adjacent")
     return t.data_ptr(), n, width, max(s0, width)
 
