@@ -6,8 +6,9 @@
 // 128. Per unit, with the unit's blocks' scales ks and vs and c = scale log2(e):
 //   S = Q K^T           Q in f16 with a power of two of its own per row (exact for 16-bit rows;
 //                       f32 rows as two f16, 22 bits), K the codes, exact in f16
-//   s = c ks S,  m' = max(m, max s),  a = 2^(m - m'),  p = 2^(s - m'),  l = a l + sum p
-//   o = a o + (p vs) V  V the codes, exact in f16 and bf16; p vs in f16 (f16 rows), in two bf16
+//   s = c ks S,  m = max s,  p = 2^(s - m),  l = sum p          (of the unit alone)
+//   o = a o + b (p vs) V,  l' = a l' + b l,  m' = max(m', m),  a, b = 2^(old m' - m'), 2^(m - m')
+//                       V the codes, exact in f16 and bf16; p vs in f16 (f16 rows), in two bf16
 //                       (bf16 rows) or three (f32 rows). bf16 has f32's range: a weight that is
 //                       far below its row's largest keeps its digits.
 // The tensor core truncates its f32 sums, about 2^-25 of the sum at every 16-element step. So S
@@ -15,21 +16,30 @@
 // is added to o in registers, rounded, with the rescale.
 //
 // Work: MMA time is (DIM / 16) NQ + 8 NP steps a unit against 16 for one plain product pair; the
-// exponentials are 128 x 128 a unit on 16 lanes an SM and clock, about as long as two products.
-// One CTA an SM, four warpgroups, every hand-over an mbarrier:
-//   0  softmax: a thread a row; S from TMEM to registers, p's parts back over S
-//   1  accumulation: a thread a row; the unit's P V from TMEM, o in registers; writes the output
-//   2  conversion: codes from the raw rings to f16 / bf16 operand tiles (128-byte swizzle), and
-//      the query rows of a new tile
-//   3  a warp that issues the MMAs, one that loads keys and one that loads values (a bulk copy
-//      for 16 tokens each, kv_cache.cuh)
-// S is double-buffered: the order of the MMAs is S(i + 1), P V(i), S(i + 2), .. so that they run
-// under the softmax. One K operand tile is enough (K(i + 2) is converted during P V(i)), and for
-// f32 rows, whose products take longer, one V tile (V(i + 1) during S(i + 2)).
+// exponentials are 128 x 128 a unit on 16 lanes an SM and clock, about as long as two products;
+// and the issue slots: about 850 (16-bit rows) to 1200 (f32) a softmax warp, 500 a conversion
+// warp and 200 an accumulation warp a unit, on each of the SM's four sub-partitions.
+// One CTA an SM, six warpgroups, every hand-over an mbarrier:
+//   0, 1  the query rows of a new tile; softmax, every other unit each (a unit's needs nothing of
+//         the one before): a thread a row; S from TMEM, p's parts back over it
+//   2     accumulation: a thread a row; the unit's P V from TMEM, o in registers; the output
+//   3, 4  conversion of keys, of values: codes from the raw rings to f16 / bf16 operand tiles
+//         (128-byte swizzle)
+//   5     a warp that issues the MMAs, one that loads keys and one that loads values (a bulk copy
+//         for 16 tokens each, kv_cache.cuh), and one that finds this CTA's pieces of tiles and
+//         hands them to the others
+// NB buffers of S: the order of the MMAs is S(i + NB - 1), P V(i), S(i + NB), .. so that they run
+// under the softmax. One K operand tile is enough (K(i) is converted while other MMAs run), and
+// for f32 rows, whose products take longer, one V tile (V(i + 1) during S(i + 2)).
 //
-// Tiles of all sequences and kv heads form one line of units, cut into equal parts, one a CTA; a
-// tile that spans CTAs is put together from the workspace by the last of them to finish, in the
-// order of the line (as in kv_attn.cu).
+// The code has to be small: beyond about 32 KB of loops, and 128 KB in all, instruction fetches
+// take longer than the instructions (measured: 2 and 6 clocks each). So loops are rolled, what
+// happens once a tile is there once, and the pieces are found by one warp.
+//
+// Tiles of all sequences and kv heads form one line of units (and of TILE_COST more a tile, for
+// what its start and end take), cut into equal parts, one a CTA; a tile that spans CTAs is put
+// together from the workspace by the last of them to finish, in the order of the line (as in
+// kv_attn.cu).
 #include "kv_attn.cuh"
 #include "ptx.cuh"
 
@@ -42,11 +52,18 @@ namespace {
 constexpr int TM = 128;        // query rows of a tile
 constexpr int TN = 128;        // cached tokens of a unit
 constexpr int GROUPS = TN / KV_GROUP;
-constexpr int THREADS = 512;
+constexpr int THREADS = 768;
+constexpr int TILE_COST = 7;   // of a tile's start and end, in units (measured: 7 best of 2, 4, 7, 10)
 constexpr int RAW = 2;         // raw rings of codes, units
 constexpr int SC = 8;          // ring of block scales, units
-constexpr int REGS_SOFT = 136, REGS_SUM = 208, REGS_CONV = 96, REGS_REST = 72;  // of a warpgroup
-static_assert(REGS_SOFT + REGS_SUM + REGS_CONV + REGS_REST <= 4 * 128, "what the launch holds");
+constexpr int REGS_SOFT = 88, REGS_SUM = 184, REGS_CONV = 40, REGS_REST = 40;  // of a warpgroup
+constexpr int REGS_LAUNCH = 80;  // what the launch gives each
+static_assert(2 * REGS_SOFT + REGS_SUM + 2 * REGS_CONV + REGS_REST <= 6 * REGS_LAUNCH &&
+                  6 * 128 * REGS_LAUNCH <= 65536,
+              "the shares come from what the launch holds");
+static_assert(REGS_SOFT >= REGS_LAUNCH && REGS_SUM >= REGS_LAUNCH && REGS_CONV <= REGS_LAUNCH &&
+                  REGS_REST <= REGS_LAUNCH,
+              "an increase must not go down, nor a decrease up: either is an illegal instruction");
 
 // TYPE: the rows'. NQ: f16 parts of a query element; NP: parts of p; F16: p and V are f16 (else
 // bf16).
@@ -60,9 +77,21 @@ struct PreCfg {
     static constexpr int KA = (DIM + 63) / 64;       // 64-element swizzle atoms of a head
     static constexpr int NV = NQ == 2 ? 1 : 2;       // V buffers
     static constexpr int SIDE_BYTES = 16 * DIM;      // a group's keys, or its values
-    static constexpr int S_COLS = 192;               // TMEM columns of an S / P buffer
-    static constexpr int O_COL = 2 * S_COLS;
-    static_assert(DIM <= 128 && NP * TN / 2 <= S_COLS, "TMEM: two S / P buffers and one o");
+    // TMEM: NB buffers of S, then of p's parts (a third part stands behind the 128 columns of S)
+    static constexpr int S_COLS = NP == 3 ? 192 : 128;
+    static constexpr int NB = NP == 3 ? 2 : 3;
+    static constexpr int O_COL = NB * S_COLS;
+    static_assert(DIM <= 128 && O_COL + 128 <= 512, "TMEM");
+};
+
+// Units key0 / TN .. + n of one tile (n = 0: no more pieces).
+struct Piece {
+    int n, key0;
+    int row0, head, q0, nq;      // the tile's first row; the sequence's query tokens
+    int pos0, len;               // position of query token 0; cached tokens
+    int lo, hi;                  // tokens that some row of the tile sees
+    int all_lo, all_hi;          // tokens that every row sees
+    int seq, cta0, cta1;         // the CTAs that have units of the tile
 };
 
 template <class C>
@@ -74,16 +103,14 @@ struct PreSmem {
     alignas(128) uint8_t raw_v[RAW][GROUPS * C::SIDE_BYTES];
     float2 sc[SC][GROUPS];   // (ks, vs)
     uint32_t valid[SC];      // bit: this group of the unit is there
-    float alpha[4][TM];
-    float row_scale[TM], fin_m[TM], fin_l[TM];
-    uint64_t rk_full[RAW], rk_empty[RAW], rv_full[RAW], rv_empty[RAW], sc_full[SC], k_full,
-        k_empty, v_full[C::NV], v_empty[C::NV], q_full, q_empty, s_full[2], p_full[2], o_full, o_empty, a_full[4],
-        fin_full, fin_empty, merge, done;
-    long long warp_sum[THREADS / 32];
-    long long line_total, first_start;
-    int first_seq, first_tile, first_head;
+    float2 stats[4][TM];     // (m, l) of a unit's rows
+    float row_scale[TM];
+    uint64_t rk_full[RAW], rk_empty[RAW], rv_full[RAW], rv_empty[RAW], k_full, k_empty,
+        v_empty[C::NV], q_full, q_empty, s_full[C::NB], pv_ready[4], o_full, merge, done;
+    Piece pieces[2];
+    uint64_t piece_full[2], piece_empty[2];
     uint32_t tmem;
-    int abort_flag, is_last, n_big;
+    int abort_flag, is_last;
 };
 
 // ---------------------------------------------------------------- PTX
@@ -121,23 +148,14 @@ constexpr uint32_t idesc_f16(int n, bool bf16) {
 // 32 lanes x 32 columns: thread = lane
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-        "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+        "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
           "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
           "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
           "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
           "=r"(r[31])
-        : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t *r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-        "%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t *r) {
@@ -149,6 +167,15 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t *r) {
 __device__ __forceinline__ void tmem_st_wait() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
+// One lane of the warp, which the compiler knows to be one: what the MMAs take from uniform
+// registers then stays in them.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(~0u, x, 0); }
 __device__ __forceinline__ void proxy_fence() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -212,68 +239,33 @@ __device__ __forceinline__ uint32_t pair_bf16(uint32_t w, int first) {
 
 // One tile: rows row0 .. of the sequence; units first .. first + units of 128 tokens.
 struct Tile {
-    int row0, first, units, pos0;  // pos0: position of query token 0
+    int row0, first, units, pos0, lo, hi;
 };
 __device__ __forceinline__ Tile tile_of(const AttnParams &p, const AttnSeq &s, int tile) {
     Tile t;
     t.row0 = tile * TM;
     t.pos0 = s.len - s.nq;
     const int last = (int)min((long long)t.row0 + TM - 1, (long long)s.nq * p.group - 1) / p.group;
-    const int hi = p.causal ? max(0, min(s.len, t.pos0 + last + 1)) : s.len;
-    int lo = 0;
+    t.hi = p.causal ? max(0, min(s.len, t.pos0 + last + 1)) : s.len;
+    t.lo = 0;
     if (p.window)
-        lo = (int)min(max((long long)t.pos0 + t.row0 / p.group - p.window + 1, 0ll),
-                      (long long)hi);
-    t.first = lo / TN;
-    t.units = max(1, (hi + TN - 1) / TN - t.first);
+        t.lo = (int)min(max((long long)t.pos0 + t.row0 / p.group - p.window + 1, 0ll),
+                        (long long)t.hi);
+    t.first = t.lo / TN;
+    t.units = max(1, (t.hi + TN - 1) / TN - t.first);
     return t;
 }
 __device__ __forceinline__ int tiles_of(const AttnParams &p, const AttnSeq &s) {
     return (int)(((long long)s.nq * p.group + TM - 1) / TM);
 }
-
-// A CTA's part of the line: pieces of tiles. Order: sequence, tile from the last (the longest of
-// a causal prompt) to the first, kv head.
-struct Cursor {
-    long long u, end, start;  // this CTA's units left; the line's unit where the tile starts
-    int seq, tile, head;
-    AttnSeq s;
-    Tile t;
-    int c0, n;  // the piece: units c0 .. c0 + n of the tile
-};
-template <class C>
-__device__ __forceinline__ bool cursor_first(const AttnParams &p, const PreSmem<C> &sm,
-                                             long long u0, long long u1, Cursor &k) {
-    k.u = u0;
-    k.end = u1;
-    k.start = sm.first_start;
-    k.seq = sm.first_seq;
-    k.tile = sm.first_tile;
-    k.head = sm.first_head;
-    k.s = attn_seq(p, k.seq);
-    k.t = tile_of(p, k.s, k.tile);
-    k.c0 = (int)(u0 - k.start);
-    k.n = (int)min((long long)(k.t.units - k.c0), u1 - u0);
-    return true;
-}
-__device__ __forceinline__ bool cursor_next(const AttnParams &p, Cursor &k) {
-    k.u += k.n;
-    if (k.u >= k.end) return false;
-    k.start += k.t.units;
-    if (++k.head == p.kv_heads) {
-        k.head = 0;
-        if (--k.tile < 0) {
-            do {
-                k.seq++;
-                k.s = attn_seq(p, k.seq);
-            } while (k.s.nq == 0);
-            k.tile = tiles_of(p, k.s) - 1;
-        }
-        k.t = tile_of(p, k.s, k.tile);
-    }
-    k.c0 = 0;
-    k.n = (int)min((long long)k.t.units, k.end - k.u);
-    return true;
+// A warp: the line's length up to tile `from` (counted from the last: tile tiles - 1 first) of
+// one sequence and kv head.
+__device__ __forceinline__ long long line_of(const AttnParams &p, const AttnSeq &s, int from,
+                                             int lane) {
+    long long x = 0;
+    for (int r = from + lane; r < tiles_of(p, s); r += 32) x += tile_of(p, s, r).units + TILE_COST;
+    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(~0u, x, d);
+    return x;
 }
 
 // Query rows in, output rows out.
@@ -284,30 +276,49 @@ __device__ __forceinline__ float load1(const void *q, size_t i) {
         return __half2float(__ldg(static_cast<const __half *>(q) + i));
     else return __bfloat162float(__ldg(static_cast<const __nv_bfloat16 *>(q) + i));
 }
+// Elements i .. i + 15 as f32 bits; those from n on are 0 (n a multiple of 8).
 template <int TYPE>
-__device__ __forceinline__ float4 load4(const AttnParams &p, size_t i) {
-    if (!p.q_vec)
-        return make_float4(load1<TYPE>(p.q, i), load1<TYPE>(p.q, i + 1), load1<TYPE>(p.q, i + 2),
-                           load1<TYPE>(p.q, i + 3));
-    if constexpr (TYPE == JKB_F32) {
-        return __ldg(reinterpret_cast<const float4 *>((const float *)p.q + i));
-    } else {
-        const uint2 v = __ldg(reinterpret_cast<const uint2 *>((const uint16_t *)p.q + i));
-        if constexpr (TYPE == JKB_F16) {
-            const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&v.x));
-            const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
-            return make_float4(a.x, a.y, b.x, b.y);
+__device__ __forceinline__ void load16(const AttnParams &p, size_t i, int n, uint32_t (&x)[16]) {
+#pragma unroll
+    for (int k = 0; k < 16; k++) x[k] = 0;
+    if (!p.q_vec) {
+#pragma unroll
+        for (int k = 0; k < 16; k++)
+            if (k < n) x[k] = __float_as_uint(load1<TYPE>(p.q, i + k));
+        return;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (8 * h >= n) continue;
+        if constexpr (TYPE == JKB_F32) {
+            const uint4 *q = reinterpret_cast<const uint4 *>((const float *)p.q + i + 8 * h);
+            const uint4 a = __ldg(q), b = __ldg(q + 1);
+            x[8 * h] = a.x, x[8 * h + 1] = a.y, x[8 * h + 2] = a.z, x[8 * h + 3] = a.w;
+            x[8 * h + 4] = b.x, x[8 * h + 5] = b.y, x[8 * h + 6] = b.z, x[8 * h + 7] = b.w;
         } else {
-            return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u),
-                               __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xFFFF0000u));
+            const uint4 a =
+                __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)p.q + i + 8 * h));
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if constexpr (TYPE == JKB_F16) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
+                    x[8 * h + 2 * k] = __float_as_uint(f.x);
+                    x[8 * h + 2 * k + 1] = __float_as_uint(f.y);
+                } else {
+                    x[8 * h + 2 * k] = w[k] << 16;
+                    x[8 * h + 2 * k + 1] = w[k] & 0xFFFF0000u;
+                }
+            }
         }
     }
 }
 template <int TYPE>
-__device__ __forceinline__ void store8(const AttnParams &p, size_t i, const float (&x)[8]) {
+__device__ __forceinline__ void store8(const AttnParams &p, size_t i, const float (&x)[8],
+                                       bool vec) {
     if constexpr (TYPE == JKB_F32) {
         float *o = static_cast<float *>(p.out) + i;
-        if (p.out_vec) {
+        if (vec) {
             *reinterpret_cast<float4 *>(o) = make_float4(x[0], x[1], x[2], x[3]);
             *reinterpret_cast<float4 *>(o + 4) = make_float4(x[4], x[5], x[6], x[7]);
         } else {
@@ -327,7 +338,7 @@ __device__ __forceinline__ void store8(const AttnParams &p, size_t i, const floa
             }
         }
         uint16_t *o = static_cast<uint16_t *>(p.out) + i;
-        if (p.out_vec) {
+        if (vec) {
             *reinterpret_cast<uint4 *>(o) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
 #pragma unroll
@@ -356,97 +367,94 @@ __device__ __forceinline__ float scale_f16(float vs, int vexp) {
 }
 
 // One unit of one row (thread): S from TMEM at ts, scaled by rs ks and masked to tokens lo .. hi
-// of the unit, into the row's running m and l; alpha, the factor of what was summed before, goes
-// to shared memory as soon as it is known. p's parts go back to TMEM over S: of the 16 columns of
-// a group of tokens, the first 8 take part 0, the last 8 part 1; part 2 stands behind S.
-// S is read twice (maximum, then weights), a group at a time, so that the loops stay rolled: with
-// more unrolling the roles' loops together outgrow the SM's instruction cache, and every unit
-// fetches them anew (unrolled over 128 columns, four times slower).
+// of the unit; returns (m, l). p's parts go back to TMEM over S: of the 16 columns of a group of
+// tokens, the first 8 take part 0, the last 8 part 1; part 2 stands behind S.
+// S is read twice (maximum, then weights), 32 columns at a time: loops stay rolled where they can: with more unrolling the roles'
+// code outgrows the SM's instruction cache, and every unit fetches it anew (unrolled over 128
+// columns, four times slower).
+// rs and ks are not negative (a negative softmax scale's sign is in Q).
 template <class C, bool MASKED>
-__device__ __forceinline__ void softmax_unit(uint32_t ts, const float2 *sc, uint32_t valid,
-                                             float rs, int lo, int hi, float &m, float &l,
-                                             float *alpha_out, uint64_t *alpha_bar) {
+__device__ __forceinline__ float2 softmax_unit(uint32_t ts, const float2 *sc, uint32_t valid,
+                                               float rs, int lo, int hi) {
     constexpr int NP = C::NP;
-    uint32_t r[16];
-    tmem_ld16(ts, r);
-    float top[2] = {m, -INFINITY};
+    float top = -INFINITY;
+    uint32_t r[32];
+    tmem_ld32(ts, r);
 #pragma unroll 1
-    for (int g = 0; g < GROUPS; g++) {
-        const float f = rs * sc[g].x;
-        uint64_t x[8];
+    for (int h = 0; h < 4; h++) {
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = mul2(pk2(r[2 * i], r[2 * i + 1]), pkf(f, f));
-        tmem_ld16(ts + 16 * ((g + 1) % GROUPS), r);
+        for (int k = 0; k < 2; k++) {
+            float t2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            float u, w;
-            upk2(x[i], u, w);
-            if (MASKED) {
-                const int t = 16 * g + 2 * i;
-                const bool on = (valid >> g) & 1;
-                u = on && t >= lo && t < hi ? u : -INFINITY;
-                w = on && t + 1 >= lo && t + 1 < hi ? w : -INFINITY;
+            for (int i = 0; i < 8; i++) {
+                float u = __uint_as_float(r[16 * k + 2 * i]);
+                float w = __uint_as_float(r[16 * k + 2 * i + 1]);
+                if (MASKED) {
+                    const int t = 32 * h + 16 * k + 2 * i;
+                    const bool on = (valid >> (2 * h + k)) & 1;
+                    u = on && t >= lo && t < hi ? u : -INFINITY;
+                    w = on && t + 1 >= lo && t + 1 < hi ? w : -INFINITY;
+                }
+                t2[i & 1] = fmaxf(t2[i & 1], fmaxf(u, w));
             }
-            top[i & 1] = fmaxf(top[i & 1], fmaxf(u, w));
+            const float raw = fmaxf(t2[0], t2[1]);
+            top = fmaxf(top, raw == -INFINITY ? raw : raw * (rs * sc[2 * h + k].x));
         }
+        tmem_ld32(ts + 32 * ((h + 1) & 3), r);
     }
-    const float mn = fmaxf(top[0], top[1]);
-    const float ref = mn == -INFINITY ? 0.0f : mn;
-    const float alpha = ex2(m - ref);
-    m = mn;
-    *alpha_out = alpha;
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(alpha_bar);
+    const float ref = top == -INFINITY ? 0.0f : top;
     int vexp = 0;
     if (C::F16) vexp = unit_vexp(sc, valid);
-    const uint64_t nref = pkf(-ref, -ref);
+    const uint64_t nref = pkf(-ref, -ref), minus = pkf(-1.0f, -1.0f);
     uint64_t sum = 0;
 #pragma unroll 1
-    for (int g = 0; g < GROUPS; g++) {
-        const float f = rs * sc[g].x, vs = C::F16 ? scale_f16(sc[g].y, vexp) : sc[g].y;
-        uint64_t x[8];
+    for (int h = 0; h < 4; h++) {
         tmem_ld_wait();
-        // (a product and a sum, rounded as in the first pass: the largest is 2^0 exactly)
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = mul2(pk2(r[2 * i], r[2 * i + 1]), pkf(f, f));
-        if (g + 1 < GROUPS) tmem_ld16(ts + 16 * (g + 1), r);
-        uint32_t part[NP][8];
+        for (int k = 0; k < 2; k++) {
+            const int g = 2 * h + k;
+            const float f = rs * sc[g].x, vs = C::F16 ? scale_f16(sc[g].y, vexp) : sc[g].y;
+            uint32_t part[NP][8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            float u, w;
-            upk2(add2(x[i], nref), u, w);
-            if (MASKED) {
-                const int t = 16 * g + 2 * i;
-                const bool on = (valid >> g) & 1;
-                u = on && t >= lo && t < hi ? u : -INFINITY;
-                w = on && t + 1 >= lo && t + 1 < hi ? w : -INFINITY;
-            }
-            uint64_t e = pkf(ex2(u), ex2(w));
-            sum = add2(sum, e);
-            e = mul2(e, pkf(vs, vs));
-#pragma unroll
-            for (int k = 0; k < NP; k++) {
+            for (int i = 0; i < 8; i++) {
+                float u, w;
+                upk2(fma2(pk2(r[16 * k + 2 * i], r[16 * k + 2 * i + 1]), pkf(f, f), nref), u, w);
+                if (MASKED) {
+                    const int t = 16 * g + 2 * i;
+                    const bool on = (valid >> g) & 1;
+                    u = on && t >= lo && t < hi ? u : -INFINITY;
+                    w = on && t + 1 >= lo && t + 1 < hi ? w : -INFINITY;
+                }
+                uint64_t e = pkf(ex2(u), ex2(w));
+                sum = add2(sum, e);
+                e = mul2(e, pkf(vs, vs));
                 upk2(e, u, w);
                 if (C::F16) {
                     const __half2 y = __floats2half2_rn(u, w);
-                    part[k][i] = *reinterpret_cast<const uint32_t *>(&y);
+                    part[0][i] = *reinterpret_cast<const uint32_t *>(&y);
                 } else {
+                    // all parts but the last are cut off, not rounded: the upper halves
+#pragma unroll
+                    for (int j = 0; j < NP - 1; j++) {
+                        const uint32_t a = __float_as_uint(u), b = __float_as_uint(w);
+                        part[j][i] = __byte_perm(a, b, 0x7632);
+                        e = fma2(pk2(a & 0xFFFF0000u, b & 0xFFFF0000u), minus, e);
+                        upk2(e, u, w);
+                    }
                     const __nv_bfloat162 y = __floats2bfloat162_rn(u, w);
-                    part[k][i] = *reinterpret_cast<const uint32_t *>(&y);
-                    if (k < NP - 1)
-                        e = add2(e, pk2((part[k][i] << 16) ^ 0x80000000u,
-                                        (part[k][i] & 0xFFFF0000u) ^ 0x80000000u));
+                    part[NP - 1][i] = *reinterpret_cast<const uint32_t *>(&y);
                 }
             }
+            tmem_st8(ts + 16 * g, part[0]);
+            if (NP > 1) tmem_st8(ts + 16 * g + 8, part[NP > 1 ? 1 : 0]);
+            if (NP > 2) tmem_st8(ts + TN + 8 * g, part[NP - 1]);
         }
-        tmem_st8(ts + 16 * g, part[0]);
-        if (NP > 1) tmem_st8(ts + 16 * g + 8, part[NP > 1 ? 1 : 0]);
-        if (NP > 2) tmem_st8(ts + TN + 8 * g, part[NP - 1]);
+        if (h < 3) tmem_ld32(ts + 32 * (h + 1), r);
     }
     float su, sw;
     upk2(sum, su, sw);
-    l = fmaf(l, alpha, su + sw);
+    return make_float2(top, su + sw);
 }
 
 template <class C>
@@ -461,36 +469,29 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     if (tid == 0) {
         sm.abort_flag = 0;
-        sm.n_big = 0;
         for (int i = 0; i < RAW; i++) {
             mbar_init(&sm.rk_full[i], 1);
             mbar_init(&sm.rk_empty[i], 4);
             mbar_init(&sm.rv_full[i], 1);
             mbar_init(&sm.rv_empty[i], 4);
         }
-        for (int i = 0; i < SC; i++) mbar_init(&sm.sc_full[i], 1);
         mbar_init(&sm.k_full, 4);
         mbar_init(&sm.k_empty, 1);
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&sm.s_full[i], 1);
-            mbar_init(&sm.p_full[i], 4);
-        }
-        for (int i = 0; i < NV; i++) {
-            mbar_init(&sm.v_full[i], 4);
-            mbar_init(&sm.v_empty[i], 1);
-        }
-        for (int i = 0; i < 4; i++) mbar_init(&sm.a_full[i], 4);
-        mbar_init(&sm.q_full, 4);
-        mbar_init(&sm.q_empty, 5);
+        for (int i = 0; i < C::NB; i++) mbar_init(&sm.s_full[i], 1);
+        for (int i = 0; i < NV; i++) mbar_init(&sm.v_empty[i], 1);
+        for (int i = 0; i < 4; i++) mbar_init(&sm.pv_ready[i], 12);
+        mbar_init(&sm.q_full, 8);
+        mbar_init(&sm.q_empty, 9);
         mbar_init(&sm.o_full, 1);
-        mbar_init(&sm.o_empty, 4);
-        mbar_init(&sm.fin_full, 4);
-        mbar_init(&sm.fin_empty, 4);
         mbar_init(&sm.merge, 4);
         mbar_init(&sm.done, 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sm.piece_full[i], 1);
+            mbar_init(&sm.piece_empty[i], 23);  // every other warp
+        }
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (warp == 12) {
+    if (warp == 20) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(&sm.tmem)),
                      "r"(512)
@@ -503,328 +504,105 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncthreads();
     tc_fence_after();
 
-    // ---- this CTA's part of the line (the operand buffers are scratch until the roles start):
-    // units a sequence, by its thread or, where it has many tiles, by a warp; then a block scan
-    {
-        long long *sum = reinterpret_cast<long long *>(&sm.q[0][0][0]);  // [n_seqs]
-        int *big = reinterpret_cast<int *>(sum + p.n_seqs);              // [n_seqs]
-        static_assert(offsetof(PreSmem<C>, sc) >= 12 * JKB_KV_MAX_SEQS, "scratch");
-        const int per_t = (p.n_seqs + THREADS - 1) / THREADS;
-        const int a = min(tid * per_t, p.n_seqs), b = min(a + per_t, p.n_seqs);
-        for (int i = a; i < b; i++) {
-            const AttnSeq s = attn_seq(p, i);
-            const int tiles = tiles_of(p, s);
-            long long x = 0;
-            if (tiles <= 4)
-                for (int r = 0; r < tiles; r++) x += tile_of(p, s, r).units;
-            else
-                big[atomicAdd(&sm.n_big, 1)] = i;
-            sum[i] = x * p.kv_heads;
-        }
-        __syncthreads();
-        for (int j = warp; j < sm.n_big; j += THREADS / 32) {
-            const AttnSeq s = attn_seq(p, big[j]);
-            const int tiles = tiles_of(p, s);
-            long long x = 0;
-            for (int r = lane; r < tiles; r += 32) x += tile_of(p, s, r).units;
-            for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(~0u, x, d);
-            if (lane == 0) sum[big[j]] = x * p.kv_heads;
-        }
-        __syncthreads();
-        long long mine = 0;
-        for (int i = a; i < b; i++) mine += sum[i];
-        long long inc = mine;
-        for (int d = 1; d < 32; d <<= 1) {
-            const long long x = __shfl_up_sync(~0u, inc, d);
-            if (lane >= d) inc += x;
-        }
-        if (lane == 31) sm.warp_sum[warp] = inc;
-        __syncthreads();
-        long long at = inc - mine, total = 0;
-        for (int w = 0; w < THREADS / 32; w++) {
-            if (w < warp) at += sm.warp_sum[w];
-            total += sm.warp_sum[w];
-        }
-        if (tid == 0) sm.line_total = total;
-        const long long per = (total + gridDim.x - 1) / gridDim.x;
-        const long long u0 = min(per * blockIdx.x, total);
-        for (int i = a; i < b; i++) {
-            if (sum[i] && u0 >= at && u0 < at + sum[i]) {
-                sm.first_seq = i;
-                sm.first_start = at;  // of the sequence, until the tile is found
-            }
-            at += sum[i];
-        }
-        __syncthreads();
-        if (warp == 0 && u0 < total) {
-            const int seq = sm.first_seq;
-            const AttnSeq s = attn_seq(p, seq);
-            long long left = u0 - sm.first_start, start = sm.first_start;
-            for (int r = tiles_of(p, s) - 1;; r -= 32) {
-                const int units = r - lane >= 0 ? tile_of(p, s, r - lane).units : 0;
-                long long x = (long long)units * p.kv_heads, upto = x;
-                for (int d = 1; d < 32; d <<= 1) {
-                    const long long y = __shfl_up_sync(~0u, upto, d);
-                    if (lane >= d) upto += y;
-                }
-                const unsigned hit = __ballot_sync(~0u, left < upto);
-                if (hit) {
-                    if (lane == __ffs(hit) - 1) {
-                        const long long in = left - (upto - x);
-                        sm.first_tile = r - lane;
-                        sm.first_head = (int)(in / units);
-                        sm.first_start = start + (upto - x) + in / units * units;
-                    }
-                    break;
-                }
-                const long long all = __shfl_sync(~0u, upto, 31);
-                left -= all;
-                start += all;
-            }
-        }
-        proxy_fence();  // the scratch becomes the target of bulk copies
-        __syncthreads();
-    }
-    const long long total = sm.line_total, per = (total + gridDim.x - 1) / gridDim.x;
-    const long long u0 = min(per * blockIdx.x, total), u1 = min(u0 + per, total);
     const uint32_t tmem = sm.tmem;
-    Cursor cur;
-    bool more = u0 < u1;
-    if (more) cursor_first<C>(p, sm, u0, u1, cur);
     // a warp's wait: all of its lanes go on, or (after the limit, or an abort) none
     auto wait = [&](uint64_t *bar, uint32_t parity) {
         return __all_sync(~0u, mbar_wait_short(bar, parity & 1, abort_flag, p.err)) != 0;
     };
 
-    if (wg == 0) {
-        // ------------------------------------------------------------ softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFT));
-        const uint32_t tl = tmem + ((uint32_t)(warp * 32) << 16);
-        const int row = tid;  // of the tile
-        uint32_t it = 0, piece = 0;
-        for (; more; more = cursor_next(p, cur), piece++) {
-            if (!wait(&sm.q_full, piece)) goto out;
-            const float rs = sm.row_scale[row];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.q_empty);
-            const int tok = (cur.t.row0 + row) / p.group, pos = cur.t.pos0 + tok;
-            const int hi = p.causal ? min(cur.s.len, pos + 1) : cur.s.len;
-            const int lo = p.window ? max(0, pos - p.window + 1) : 0;
-            // tokens that every row of the tile sees
-            const int pos_a = cur.t.pos0 + cur.t.row0 / p.group;
-            const int pos_b = cur.t.pos0 + (cur.t.row0 + TM - 1) / p.group;
-            const int all_hi = p.causal ? min(cur.s.len, pos_a + 1) : cur.s.len;
-            const int all_lo = p.window ? pos_b - p.window + 1 : 0;
-            float m = -INFINITY, l = 0.0f;
-            for (int c = 0; c < cur.n; c++, it++) {
-                const int b = it & 1;
-                if (!wait(&sm.sc_full[it % SC], it / SC) || !wait(&sm.s_full[b], it >> 1))
-                    goto out;
-                tc_fence_after();
-                const int key0 = (cur.t.first + cur.c0 + c) * TN;
-                const uint32_t valid = sm.valid[it % SC];
-                const bool masked = key0 < all_lo || key0 + TN > all_hi || valid != 0xFFu;
-                const float2 *sc = sm.sc[it % SC];
-                const uint32_t ts = tl + b * C::S_COLS;
-                if (masked)
-                    softmax_unit<C, true>(ts, sc, valid, rs, lo - key0, hi - key0, m, l,
-                                          &sm.alpha[it & 3][row], &sm.a_full[it & 3]);
-                else
-                    softmax_unit<C, false>(ts, sc, valid, rs, 0, TN, m, l,
-                                           &sm.alpha[it & 3][row], &sm.a_full[it & 3]);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.p_full[b]);
-            }
-            if (!wait(&sm.fin_empty, piece + 1)) goto out;
-            sm.fin_m[row] = m;
-            sm.fin_l[row] = l;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.fin_full);
-        }
-    } else if (wg == 1) {
-        // ------------------------------------------------------------ accumulation and output
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SUM));
-        const int row = tid - 128;
-        const uint32_t tl = tmem + ((uint32_t)((warp - 4) * 32) << 16) + C::O_COL;
-        uint32_t it = 0, piece = 0, merges = 0;
-        for (; more; more = cursor_next(p, cur), piece++) {
-            uint64_t o[DIM / 2];  // pairs of columns
-#pragma unroll
-            for (int i = 0; i < DIM / 2; i++) o[i] = 0;
-            for (int c = 0; c < cur.n; c++, it++) {
-                if (!wait(&sm.a_full[it & 3], it >> 2)) goto out;
-                const float alpha = sm.alpha[it & 3][row];
-                const uint64_t al = pkf(alpha, alpha);
-                float up = 1.0f;  // (a power of two that flushes to 0 is below f16's smallest)
-                if (C::F16) up = ex2((float)(unit_vexp(sm.sc[it % SC], sm.valid[it % SC]) - 14));
-                if (!wait(&sm.o_full, it)) goto out;
-                tc_fence_after();
-                uint32_t r[2][32];
-                tmem_ld32(tl, r[0]);
-#pragma unroll
-                for (int q = 0; q < DT; q++) {
-                    tmem_ld_wait();
-                    if (q + 1 < DT) tmem_ld32(tl + 32 * (q + 1), r[(q + 1) & 1]);
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        uint64_t x = pk2(r[q & 1][2 * i], r[q & 1][2 * i + 1]);
-                        if (C::F16) x = mul2(x, pkf(up, up));
-                        o[16 * q + i] = fma2(o[16 * q + i], al, x);
-                    }
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.o_empty);
-            }
-            if (!wait(&sm.fin_full, piece)) goto out;
-            float m = sm.fin_m[row], l = sm.fin_l[row];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.fin_empty);
+    // two barriers at once
+    auto wait2 = [&](uint64_t *bar0, uint32_t parity0, uint64_t *bar1, uint32_t parity1) {
+        const bool a = mbar_try(bar0, parity0 & 1), b = mbar_try(bar1, parity1 & 1);
+        return __all_sync(~0u, a && b) || (wait(bar0, parity0) && wait(bar1, parity1));
+    };
+    // the next piece: waits for it, copies it and gives its slot back; false at the end
+    uint32_t pieces = 0;
+    Piece cur;
+    auto next_piece = [&](bool &ok) {
+        const uint32_t i = pieces & 1;
+        ok = wait(&sm.piece_full[i], pieces >> 1);
+        cur = sm.pieces[i];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.piece_empty[i]);
+        pieces++;
+        return ok && cur.n > 0;
+    };
+    bool ok = true;
 
-            const int cta0 = (int)(cur.start / per);
-            const int cta1 = (int)((cur.start + cur.t.units - 1) / per);
-            if (cta0 != cta1) {
-                auto slot_of = [&](int cta) {
-                    const int slot = 2 * cta + (cta == cta0 && cur.start != per * cta0 ? 1 : 0);
-                    return p.tile_partial + (size_t)slot * TM * (DIM + 2);
-                };
-                float *mine = slot_of((int)blockIdx.x);
+    // (one instruction for all warps of a group; what is taken was given back first)
+    if (wg < 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFT));
+    else if (wg == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SUM));
+    else if (wg < 5) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CONV));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_REST));
+
+    if (wg < 2) {
+        // ------------------------------------------------------------ softmax
+        const int row = tid & 127;  // of the tile
+        constexpr int QROUNDS = NQ == 2 ? 1 : 2;
+        const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        uint32_t it = 0;
+        while (next_piece(ok)) {
+            // ---- the query rows, 16 a warp: f16 parts of x times a power of two of the row ----
+            if (!wait(&sm.q_empty, pieces)) goto out;
+            // eight lanes a row, 16 dims a lane; two rounds of rows in flight
+            {
+                const int d0 = 16 * (lane & 7);
+                int rr = cur.row0 + warp * 16 + (lane >> 3), tok = rr / p.group;
+                int h = rr - tok * p.group;
+                const size_t head0 = (size_t)(cur.head * p.group);
+#pragma unroll 1
+                for (int r0 = 0; r0 < 16; r0 += 4 * QROUNDS) {
+                    uint32_t x[QROUNDS][16];
 #pragma unroll
-                for (int i = 0; i < DIM / 2; i++) {
-                    float u, w;
-                    upk2(o[i], u, w);
-                    mine[2 * i * TM + row] = u;
-                    mine[(2 * i + 1) * TM + row] = w;
-                }
-                mine[DIM * TM + row] = m;
-                mine[(DIM + 1) * TM + row] = l;
-                __threadfence();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.merge);
-                if (!wait(&sm.merge, merges++)) goto out;
-                if (tid == 128) {
-                    const int before = atomicAdd(&p.tile_counters[cta0], 1);
-                    sm.is_last = before == cta1 - cta0;
-                    if (sm.is_last) p.tile_counters[cta0] = 0;
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.merge);
-                if (!wait(&sm.merge, merges++)) goto out;
-                const bool last = *(volatile int *)&sm.is_last;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.merge);  // is_last may be written again
-                if (!wait(&sm.merge, merges++)) goto out;
-                if (!last) continue;
-                __threadfence();
-                m = -INFINITY;
-                for (int k = cta0; k <= cta1; k++)
-                    m = fmaxf(m, __ldcg(slot_of(k) + DIM * TM + row));
-                const float ref = m == -INFINITY ? 0.0f : m;
-                l = 0.0f;
-#pragma unroll
-                for (int i = 0; i < DIM / 2; i++) o[i] = 0;
-                for (int k = cta0; k <= cta1; k++) {
-                    const float *x = slot_of(k) + row;
-                    const float w = ex2(__ldcg(x + DIM * TM) - ref);
-                    l = fmaf(w, __ldcg(x + (DIM + 1) * TM), l);
-#pragma unroll
-                    for (int i = 0; i < DIM / 2; i++)
-                        o[i] = fma2(pkf(w, w), pkf(__ldcg(x + 2 * i * TM),
-                                                   __ldcg(x + (2 * i + 1) * TM)), o[i]);
-                }
-            }
-            const int rr = cur.t.row0 + row, tok = rr / p.group;
-            const int h = cur.head * p.group + rr - tok * p.group;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            if (tok < cur.s.nq) {
-                if (p.lse)
-                    p.lse[(size_t)(cur.s.q0 + tok) * p.group * p.kv_heads + h] =
-                        (m + log2f(l)) * 0.69314718055994531f;
-                const size_t at = (size_t)(cur.s.q0 + tok) * p.out_token + (size_t)h * p.out_head;
-                // column 32 c + 8 j + g of o is dim 32 c + 4 g + j
-#pragma unroll
-                for (int c = 0; c < DT; c++)
-#pragma unroll
-                    for (int g = 0; g < 8; g += 2) {
-                        const int d = 32 * c + 4 * g;
-                        float x[8];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {  // columns 8 i + g and 8 i + g + 1
-                            upk2(o[16 * c + 4 * i + g / 2], x[i], x[4 + i]);
-                            x[i] *= inv;
-                            x[4 + i] *= inv;
+                    for (int j = 0; j < QROUNDS; j++) {
+                        const size_t at = (size_t)(cur.q0 + tok) * p.q_token +
+                                          (head0 + h) * p.q_head + d0;
+                        load16<C::TYPE>(p, at, tok < cur.nq ? p.dim - d0 : 0, x[j]);
+                        h += 4;
+                        while (h >= p.group) {
+                            h -= p.group;
+                            tok++;
                         }
-                        if (d < p.dim) store8<C::TYPE>(p, at + d, x);
                     }
-            }
-            __syncwarp();
-        }
-    } else if (wg == 2) {
-        // ------------------------------------------------------------ conversion
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CONV));
-        const int ct = tid - 256, cw = warp - 8;
-        uint32_t it = 0, piece = 0;
-        for (; more; more = cursor_next(p, cur), piece++) {
-            // ---- the query rows: f16 parts of x times a power of two of the row ----
-            if (!wait(&sm.q_empty, piece + 1)) goto out;
-            // eight lanes a row, 16 dims a lane
-#pragma unroll 2
-            for (int r0 = 0; r0 < 32; r0 += 4) {
-                const int r = cw * 32 + r0 + (lane >> 3), d0 = 16 * (lane & 7);
-                const int rr = cur.t.row0 + r, tok = rr / p.group;
-                const size_t at = (size_t)(cur.s.q0 + tok) * p.q_token +
-                                  (size_t)(cur.head * p.group + rr - tok * p.group) * p.q_head;
-                float4 x[4];
-                float top = 0.0f;
-                bool fine = true;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (tok < cur.s.nq && d0 + 4 * k < p.dim)
-                        x[k] = load4<C::TYPE>(p, at + d0 + 4 * k);
-                }
+                    for (int j = 0; j < QROUNDS; j++) {
+                        const int r = warp * 16 + r0 + 4 * j + (lane >> 3);
+                        // the largest magnitude's bits; infinities and NaN are above all others
+                        uint32_t top = 0;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const float a = fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)),
-                                          fmaxf(fabsf(x[k].z), fabsf(x[k].w)));
-                    top = fmaxf(top, a);
-                    // a non-finite element makes the sum of the element times 0 a NaN
-                    fine &= x[k].x * 0.0f + x[k].y * 0.0f + x[k].z * 0.0f + x[k].w * 0.0f == 0.0f;
-                }
-                for (int d = 4; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-                const unsigned rows_fine = __ballot_sync(~0u, fine);
-                fine = ((rows_fine >> (lane & 24)) & 0xFFu) == 0xFFu;
-                // 2^e brings the largest element into [2^14, 2^15)
-                const int e = min(14 + 127 - (int)((__float_as_uint(top) >> 23) & 255), 126);
-                float up = __uint_as_float((uint32_t)(127 + e) << 23);
-                if ((lane & 7) == 0)
-                    sm.row_scale[r] = !fine ? __int_as_float(0x7FC00000)
-                                      : top == 0.0f ? 0.0f : p.scale2 / up;
-                if (64 * C::KA > d0) {
+                        for (int k = 0; k < 16; k++) top = max(top, x[j][k] & 0x7FFFFFFFu);
+                        for (int d = 4; d; d >>= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
+                        const bool fine = top < 0x7F800000u;
+                        // 2^e brings the largest element into [2^14, 2^15)
+                        const int e = min(14 + 127 - (int)(top >> 23), 126);
+                        float up = fine ? __uint_as_float((uint32_t)(127 + e) << 23) : 0.0f;
+                        if ((lane & 7) == 0)
+                            sm.row_scale[r] = !fine ? __int_as_float(0x7FC00000)
+                                              : top == 0 ? 0.0f : fabsf(p.scale2) / up;
+                        up = copysignf(up, p.scale2);
+                        if (64 * C::KA <= d0) continue;
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        float v[8] = {x[2 * h].x, x[2 * h].y, x[2 * h].z, x[2 * h].w,
-                                      x[2 * h + 1].x, x[2 * h + 1].y, x[2 * h + 1].z,
-                                      x[2 * h + 1].w};
+                        for (int i = 0; i < 2; i++) {
+                            float v[8];
 #pragma unroll
-                        for (int k = 0; k < 8; k++) v[k] = fine ? v[k] * up : 0.0f;
-                        const int ch = (2 * (lane & 7) + h) & 7;
+                            for (int k = 0; k < 8; k++)
+                                v[k] = fine ? __uint_as_float(x[j][8 * i + k]) * up : 0.0f;
+                            const int ch = (2 * (lane & 7) + i) & 7;
+                            uint8_t *dst = &sm.q[0][d0 >> 6][r * 128 + ((ch ^ (r & 7)) << 4)];
 #pragma unroll
-                        for (int k = 0; k < NQ; k++) {
-                            uint32_t w[4];
+                            for (int k = 0; k < NQ; k++) {
+                                uint32_t w[4];
 #pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const __half2 y = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-                                const float2 f = __half22float2(y);
-                                w[i] = *reinterpret_cast<const uint32_t *>(&y);
-                                v[2 * i] -= f.x;
-                                v[2 * i + 1] -= f.y;
+                                for (int t = 0; t < 4; t++) {
+                                    const __half2 y = __floats2half2_rn(v[2 * t], v[2 * t + 1]);
+                                    const float2 f = __half22float2(y);
+                                    w[t] = *reinterpret_cast<const uint32_t *>(&y);
+                                    v[2 * t] -= f.x;
+                                    v[2 * t + 1] -= f.y;
+                                }
+                                *reinterpret_cast<uint4 *>(dst + k * sizeof(sm.q[0])) =
+                                    make_uint4(w[0], w[1], w[2], w[3]);
                             }
-                            *reinterpret_cast<uint4 *>(
-                                &sm.q[k][d0 >> 6][r * 128 + ((ch ^ (r & 7)) << 4)]) =
-                                make_uint4(w[0], w[1], w[2], w[3]);
                         }
                     }
                 }
@@ -832,35 +610,212 @@ __global__ void __launch_bounds__(THREADS, 1)
             proxy_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.q_full);
-
-            // K(n), then V(n - 1)
-            for (int c = 0; c <= cur.n; c++) {
-                if (c < cur.n) {
-                    const uint32_t n = it + c;
-                    if (!wait(&sm.rk_full[n % RAW], n / RAW) || !wait(&sm.k_empty, n + 1))
-                        goto out;
-                    const uint8_t *raw = sm.raw_k[n % RAW];
-                    // unit: a token's 32 dims, its halves in the order that keeps eight lanes
-                    // (eight tokens) on eight bank groups
-#pragma unroll 1
-                    for (int u = ct; u < TN * DT; u += 128) {
-                        const int tk = u & 7, rest = u >> 3, chunk = rest % DT, hg = rest / DT;
-                        const uint8_t *src = raw + hg * 8 * DIM + chunk * 256 + tk * 32;
-                        uint8_t *dst = &sm.k[chunk >> 1][(hg * 8 + tk) * 128];
+            if (!wait(&sm.q_full, pieces - 1)) goto out;
+            const float rs = sm.row_scale[row];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.q_empty);
+            const int pos = cur.pos0 + (cur.row0 + row) / p.group;
+            const int hi = p.causal ? min(cur.len, pos + 1) : cur.len;
+            const int lo = p.window ? max(0, pos - p.window + 1) : 0;
+            const uint32_t end = it + cur.n;
+            uint32_t i = it + ((it ^ wg) & 1);
+            int key0 = cur.key0 + (int)(i - it) * TN;
+            it = end;
+            for (; i < end; i += 2, key0 += 2 * TN) {
+                const uint32_t b = i % C::NB;
+                if (!wait(&sm.s_full[b], i / C::NB)) goto out;
+                tc_fence_after();
+                const uint32_t valid = sm.valid[i % SC];
+                const float2 *sc = sm.sc[i % SC];
+                const uint32_t ts = tl + b * C::S_COLS;
+                float2 st;
+                if (key0 < cur.all_lo || key0 + TN > cur.all_hi || valid != 0xFFu)
+                    st = softmax_unit<C, true>(ts, sc, valid, rs, lo - key0, hi - key0);
+                else
+                    st = softmax_unit<C, false>(ts, sc, valid, rs, 0, TN);
+                sm.stats[i & 3][row] = st;
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.pv_ready[i & 3]);
+            }
+        }
+    } else if (wg == 2) {
+        // ------------------------------------------------------------ accumulation and output
+        const int row = tid & 127;
+        const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::O_COL;
+        uint32_t it = 0, merges = 0;
+        if (lane == 0) mbar_arrive(&sm.pv_ready[0]);  // o is free for the first unit
+        while (next_piece(ok)) {
+            uint64_t o[DIM / 2];  // pairs of columns
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const int hh = i ^ (tk >> 2);
-                            const uint4 x = *reinterpret_cast<const uint4 *>(src + 16 * hh);
-                            const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u,
-                                                   x.z ^ 0x80808080u, x.w ^ 0x80808080u};
-                            const int ch = (chunk & 1) * 4 + 2 * hh;
-                            *reinterpret_cast<uint4 *>(dst + ((ch ^ tk) << 4)) =
-                                make_uint4(pair_f16(w[0], 0x4140), pair_f16(w[0], 0x4342),
-                                           pair_f16(w[1], 0x4140), pair_f16(w[1], 0x4342));
-                            *reinterpret_cast<uint4 *>(dst + (((ch + 1) ^ tk) << 4)) =
-                                make_uint4(pair_f16(w[2], 0x4140), pair_f16(w[2], 0x4342),
-                                           pair_f16(w[3], 0x4140), pair_f16(w[3], 0x4342));
+            for (int i = 0; i < DIM / 2; i++) o[i] = 0;
+            float m = -INFINITY, l = 0.0f;
+            for (int c = 0; c < cur.n; c++, it++) {
+                if (!wait(&sm.o_full, it)) goto out;
+                tc_fence_after();
+                const float2 st = sm.stats[it & 3][row];
+                const float mn = fmaxf(m, st.x), ref = mn == -INFINITY ? 0.0f : mn;
+                const float a = ex2(m - ref), b = ex2(st.x - ref);
+                l = fmaf(l, a, b * st.y);
+                m = mn;
+                const uint64_t a2 = pkf(a, a);
+                float up = b;  // f16 (a power of two that flushes to 0 is below f16's smallest)
+                if (C::F16) up *= ex2((float)(unit_vexp(sm.sc[it % SC], sm.valid[it % SC]) - 14));
+                const uint64_t b2 = pkf(up, up);
+#pragma unroll
+                for (int q = 0; q < DT; q++) {
+                    uint32_t r[32];
+                    tmem_ld32(tl + 32 * q, r);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        o[16 * q + i] =
+                            fma2(o[16 * q + i], a2, mul2(pk2(r[2 * i], r[2 * i + 1]), b2));
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.pv_ready[(it + 1) & 3]);
+            }
+
+            const int rr = cur.row0 + row, tok = rr / p.group, h = cur.head * p.group + rr - tok * p.group;
+            const size_t at = (size_t)(cur.q0 + tok) * p.out_token + (size_t)h * p.out_head;
+            const bool on = tok < cur.nq;
+            if (cur.cta0 == cur.cta1 && p.out_vec) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                if (on) {
+                    if (p.lse)
+                        p.lse[(size_t)(cur.q0 + tok) * p.group * p.kv_heads + h] =
+                            (m + log2f(l)) * 0.69314718055994531f;
+                    // column 32 c + 8 j + g of o is dim 32 c + 4 g + j
+#pragma unroll
+                    for (int c = 0; c < DT; c++)
+#pragma unroll
+                        for (int g = 0; g < 8; g += 2) {
+                            float x[8];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {  // columns 8 i + g and 8 i + g + 1
+                                upk2(o[16 * c + 4 * i + g / 2], x[i], x[4 + i]);
+                                x[i] *= inv;
+                                x[4 + i] *= inv;
+                            }
+                            if (32 * c + 4 * g < p.dim)
+                                store8<C::TYPE>(p, at + 32 * c + 4 * g, x, true);
                         }
+                }
+                __syncwarp();
+                continue;
+            }
+            // A tile of several CTAs, each with a slot (two where a CTA starts within one such
+            // tile and ends within another), or rows that are not aligned for wide stores: by
+            // way of the workspace
+            {
+                auto slot_of = [&](int cta) {
+                    const int slot = 2 * cta + (cta == cur.cta0 ? 1 : 0);
+                    return p.tile_partial + (size_t)slot * TM * (DIM + 2) + row;
+                };
+                float *mine = slot_of((int)blockIdx.x);
+#pragma unroll
+                for (int i = 0; i < DIM / 2; i++) {
+                    float u, w;
+                    upk2(o[i], u, w);
+                    mine[2 * i * TM] = u;
+                    mine[(2 * i + 1) * TM] = w;
+                }
+                mine[DIM * TM] = m;
+                mine[(DIM + 1) * TM] = l;
+                bool last = true;
+                if (cur.cta0 != cur.cta1) {
+                    __threadfence();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.merge);
+                    if (!wait(&sm.merge, merges++)) goto out;
+                    if (row == 0) {
+                        const int before = atomicAdd(&p.tile_counters[cur.cta0], 1);
+                        sm.is_last = before == cur.cta1 - cur.cta0;
+                        if (sm.is_last) p.tile_counters[cur.cta0] = 0;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.merge);
+                    if (!wait(&sm.merge, merges++)) goto out;
+                    last = *(volatile int *)&sm.is_last;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.merge);  // is_last may be written again
+                    if (!wait(&sm.merge, merges++)) goto out;
+                    __threadfence();
+                }
+                if (!last) continue;
+                m = -INFINITY;
+                for (int k = cur.cta0; k <= cur.cta1; k++) m = fmaxf(m, __ldcg(slot_of(k) + DIM * TM));
+                const float ref = m == -INFINITY ? 0.0f : m;
+                l = 0.0f;
+                for (int k = cur.cta0; k <= cur.cta1; k++)
+                    l = fmaf(ex2(__ldcg(slot_of(k) + DIM * TM) - ref),
+                             __ldcg(slot_of(k) + (DIM + 1) * TM), l);
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                if (on && p.lse)
+                    p.lse[(size_t)(cur.q0 + tok) * p.group * p.kv_heads + h] =
+                        (m + log2f(l)) * 0.69314718055994531f;
+#pragma unroll 1
+                for (int d = 0; d < p.dim; d += 8) {
+                    float x[8] = {};
+#pragma unroll 1
+                    for (int k = cur.cta0; k <= cur.cta1; k++) {
+                        const float *slot = slot_of(k);
+                        const float w = ex2(__ldcg(slot + DIM * TM) - ref);
+                        // dim 32 c + 4 g + j is column 32 c + 8 j + g
+                        const float *col = slot + ((d & ~31) + ((d & 31) >> 2)) * TM;
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            x[i] = fmaf(w, __ldcg(col + (8 * (i & 3) + (i >> 2)) * TM), x[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[i] *= inv;
+                    if (on) store8<C::TYPE>(p, at + d, x, p.out_vec);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (wg == 3) {
+        // ------------------------------------------------------------ conversion of keys
+        const int cw = warp & 3;
+        uint32_t it = 0;
+        while (next_piece(ok)) {
+            for (int c = 0; c < cur.n; c++, it++) {
+                {
+                    const uint32_t n = it;
+                    if (!wait2(&sm.rk_full[n % RAW], n / RAW, &sm.k_empty, n + 1)) goto out;
+                    const uint8_t *raw = sm.raw_k[n % RAW];
+                    // a lane takes a token's 32 dims, their halves in the order that keeps eight
+                    // lanes (eight tokens) on eight bank groups; a warp 8 tokens, or 16 of 64 dims
+                    constexpr int PER = DT == 2 ? 2 : 1;  // eights of tokens a warp and round
+                    const int tk = lane & 7, sub = lane >> 3;
+                    const int chunk = DT == 2 ? sub & 1 : sub, eighth = DT == 2 ? sub >> 1 : 0;
+                    const int swap = tk >> 2;
+                    const int hg0 = cw * PER + eighth;
+                    const uint8_t *src = raw + hg0 * 8 * DIM + chunk * 256 + tk * 32 + 16 * swap;
+                    uint8_t *dst = &sm.k[0][0] + (chunk >> 1) * (TN * 128) + (hg0 * 8 + tk) * 128;
+                    const int ch = (chunk & 1) * 4 + 2 * swap;
+                    const int d00 = (ch ^ tk) << 4, d01 = ((ch + 1) ^ tk) << 4;
+#pragma unroll 2
+                    for (int i = 0; i < TN / 8 / (4 * PER); i++) {
+                        if (chunk < DT) {
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {  // the second half: 32 bytes of dst away
+                                const uint4 x = *reinterpret_cast<const uint4 *>(
+                                    h ? src + 16 - 32 * swap : src);
+                                const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u,
+                                                       x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+                                *reinterpret_cast<uint4 *>(dst + (d00 ^ (32 * h))) =
+                                    make_uint4(pair_f16(w[0], 0x4140), pair_f16(w[0], 0x4342),
+                                               pair_f16(w[1], 0x4140), pair_f16(w[1], 0x4342));
+                                *reinterpret_cast<uint4 *>(dst + (d01 ^ (32 * h))) =
+                                    make_uint4(pair_f16(w[2], 0x4140), pair_f16(w[2], 0x4342),
+                                               pair_f16(w[3], 0x4140), pair_f16(w[3], 0x4342));
+                            }
+                        }
+                        src += 4 * PER * 8 * DIM;
+                        dst += 4 * PER * 8 * 128;
                     }
                     proxy_fence();
                     __syncwarp();
@@ -869,17 +824,28 @@ __global__ void __launch_bounds__(THREADS, 1)
                         mbar_arrive(&sm.k_full);
                     }
                 }
-                if (c > 0) {
-                    const uint32_t n = it + c - 1;
+            }
+        }
+    } else if (wg == 4) {
+        // ------------------------------------------------------------ conversion of values
+        const int cw = warp & 3;
+        uint32_t it = 0;
+        while (next_piece(ok)) {
+            for (int c = 0; c < cur.n; c++, it++) {
+                {
+                    const uint32_t n = it;
                     const int vb = n % NV;
-                    if (!wait(&sm.rv_full[n % RAW], n / RAW) ||
-                        !wait(&sm.v_empty[vb], n / NV + 1))
+                    if (!wait2(&sm.rv_full[n % RAW], n / RAW, &sm.v_empty[vb], n / NV + 1))
                         goto out;
                     const uint8_t *raw = sm.raw_v[n % RAW];
-                    // unit: 16 tokens of four dims (4 g + j), to rows 8 j + g
+                    // a lane takes 16 tokens of four dims (4 g + j), to rows 8 j + g; a warp a group
+                    // of tokens, or two of 64 dims
+                    constexpr int PER = DT == 2 ? 2 : 1;
+                    const int g = lane & 7, sub = lane >> 3;
+                    const int chunk = DT == 2 ? sub & 1 : sub, other = DT == 2 ? sub >> 1 : 0;
 #pragma unroll 1
-                    for (int u = ct; u < GROUPS * DT * 8; u += 128) {
-                        const int g = u & 7, rest = u >> 3, chunk = rest % DT, grp = rest / DT;
+                    for (int grp = cw * PER + other; grp < GROUPS; grp += 4 * PER) {
+                        if (chunk >= DT) continue;
                         const uint8_t *src = raw + grp * C::SIDE_BYTES + chunk * 512;
                         uint32_t w[4][4];  // [t][j]
 #pragma unroll
@@ -888,9 +854,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                                 src + (t * 8 + (g ^ (2 * t))) * 16);
                             w[t][0] = x.x, w[t][1] = x.y, w[t][2] = x.z, w[t][3] = x.w;
                         }
+                        uint8_t *dst = &sm.v[vb][grp >> 2][(32 * chunk + g) * 128];
+                        const int d0 = (((grp & 3) * 2) ^ g) << 4;
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
-                            uint8_t *dst = &sm.v[vb][grp >> 2][(32 * chunk + 8 * j + g) * 128];
 #pragma unroll
                             for (int i = 0; i < 2; i++) {  // tokens 8 i .. 8 i + 7
                                 uint32_t y[4];
@@ -898,8 +865,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                                 for (int t = 0; t < 4; t++)
                                     y[t] = C::F16 ? pair_f16(w[t][j], i ? 0x4342 : 0x4140)
                                                   : pair_bf16(w[t][j], i);
-                                *reinterpret_cast<uint4 *>(
-                                    dst + ((((grp & 3) * 2 + i) ^ g) << 4)) =
+                                *reinterpret_cast<uint4 *>(dst + j * 8 * 128 + (d0 ^ (16 * i))) =
                                     make_uint4(y[0], y[1], y[2], y[3]);
                             }
                         }
@@ -908,91 +874,118 @@ __global__ void __launch_bounds__(THREADS, 1)
                     __syncwarp();
                     if (lane == 0) {
                         mbar_arrive(&sm.rv_empty[n % RAW]);
-                        mbar_arrive(&sm.v_full[vb]);
+                        mbar_arrive(&sm.pv_ready[n & 3]);
                     }
                 }
             }
-            it += cur.n;
         }
-    } else if (warp == 12) {
+    } else if (warp == 20) {
         // ------------------------------------------------------------ MMA
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_REST));
         constexpr uint32_t ID_S = idesc_f16(TN, false), ID_O = idesc_f16(DIM, !C::F16);
-        uint32_t it = 0, piece = 0;
-        auto issue_pv = [&](uint32_t i) {
-            const int b = i & 1, vb = i % NV;
-            if (!wait(&sm.p_full[b], i >> 1) || !wait(&sm.v_full[vb], i / NV) ||
-                !wait(&sm.o_empty, i + 1))
-                return false;
+        uint32_t it = 0, pv = 0;  // S and P V issued so far
+        const uint32_t ut = uniform(tmem), vd0 = uniform(desc_lo(&sm.v[0][0][0]));
+        const uint32_t kd = uniform(desc_lo(&sm.k[0][0])), qd = uniform(desc_lo(&sm.q[0][0][0]));
+        auto issue_pv = [&]() {
+            const uint32_t b = pv % C::NB, vb = pv % NV;
+            // its p, its V, and o free of the unit before
+            if (!wait(&sm.pv_ready[pv & 3], pv >> 2)) return false;
             tc_fence_after();
-            if (lane == 0) {
-                const uint32_t vd = desc_lo(&sm.v[vb][0][0]), pt = tmem + b * C::S_COLS;
-                const uint32_t od = tmem + C::O_COL;
+            const uint32_t vd = uniform(vd0 + vb * (uint32_t)(sizeof(sm.v[0]) / 16));
+            const uint32_t pt = uniform(ut + b * C::S_COLS), od = ut + C::O_COL;
+            if (elect_one()) {
                 // parts of p from the last; their columns as softmax_unit leaves them. V of step
                 // s: atom s / 4, 32 bytes a step
+                bool acc = false;
 #pragma unroll 1
                 for (int k = NP - 1; k >= 0; k--) {
-                    const uint32_t a = pt + (k == 2 ? TN : 8 * k), step = k == 2 ? 8 : 16;
-#pragma unroll
-                    for (int s = 0; s < TN / 16; s++)
-                        mma_ts(od, a + s * step, vd + (s >> 2) * (DIM * 128 / 16) + (s & 3) * 2,
-                               ID_O, s || k < NP - 1);
+                    uint32_t a = pt + (k == 2 ? TN : 8 * k), v = vd;
+                    const uint32_t step = k == 2 ? 8 : 16;
+#pragma unroll 1
+                    for (int s = 0; s < TN / 32; s++) {
+                        mma_ts(od, a, v, ID_O, acc);
+                        mma_ts(od, a + step, v + 2, ID_O, true);
+                        acc = true;
+                        a += 2 * step;
+                        v += s == 1 ? DIM * 128 / 16 - 4 : 4;
+                    }
                 }
                 tc_commit(&sm.v_empty[vb]);
                 tc_commit(&sm.o_full);
             }
             __syncwarp();
+            pv++;
             return true;
         };
-        for (; more; more = cursor_next(p, cur), piece++) {
-            if (!wait(&sm.q_full, piece)) goto out;
-            for (int c = 0; c < cur.n; c++, it++) {
-                const int b = it & 1;
-                if (!wait(&sm.k_full, it)) goto out;
+        // one loop over S's units and the P V that are left at the end, so that the code of each
+        // is there once
+        int c = 0;
+        bool more = true, fetched = false;
+        while (more || pv < it) {
+            bool s_next = more;
+            // a new tile and its query rows may be long in coming: finish what is left before them
+            if (more && c == 0) {
+                if (!fetched && (pv == it || __any_sync(~0u, mbar_try(&sm.piece_full[pieces & 1],
+                                                                      (pieces >> 1) & 1)))) {
+                    more = next_piece(ok);
+                    if (!ok) goto out;
+                    fetched = true;
+                    if (!more) continue;
+                }
+                s_next = fetched && (pv == it || __any_sync(~0u, mbar_try(&sm.q_full,
+                                                                          (pieces - 1) & 1)));
+                if (!s_next && pv == it) continue;
+            }
+            if (s_next) {
+                if ((c == 0 && !wait(&sm.q_full, pieces - 1)) || !wait(&sm.k_full, it)) goto out;
                 tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t kd = desc_lo(&sm.k[0][0]), qd = desc_lo(&sm.q[0][0][0]);
-                    const uint32_t sd = tmem + b * C::S_COLS;
+                const uint32_t sd = uniform(ut + it % C::NB * C::S_COLS);
+                const bool last_unit = c == cur.n - 1;
+                if (elect_one()) {
+                    bool acc = false;
 #pragma unroll 1
                     for (int k = NQ - 1; k >= 0; k--) {
-                        const uint32_t ad = qd + k * (C::KA * TM * 128 / 16);
-#pragma unroll
-                        for (int s = 0; s < DIM / 16; s++) {
-                            const uint32_t at = (s >> 2) * (TM * 128 / 16) + (s & 3) * 2;
-                            mma_ss(sd, ad + at, kd + at, ID_S, s || k < NQ - 1);
+                        uint32_t a = qd + k * (C::KA * TM * 128 / 16), b = kd;
+#pragma unroll 1
+                        for (int s = 0; s < DIM / 32; s++) {
+                            mma_ss(sd, a, b, ID_S, acc);
+                            mma_ss(sd, a + 2, b + 2, ID_S, true);
+                            acc = true;
+                            const uint32_t d = s == 1 ? TM * 128 / 16 - 4 : 4;
+                            a += d;
+                            b += d;
                         }
                     }
                     tc_commit(&sm.k_empty);
-                    if (c == cur.n - 1) tc_commit(&sm.q_empty);
-                    tc_commit(&sm.s_full[b]);
+                    if (last_unit) tc_commit(&sm.q_empty);
+                    tc_commit(&sm.s_full[it % C::NB]);
                 }
                 __syncwarp();
-                if (c > 0 && !issue_pv(it - 1)) goto out;
+                it++;
+                if (++c == cur.n) {
+                    c = 0;
+                    fetched = false;
+                }
+                if (it - pv < C::NB) continue;
             }
-            if (!issue_pv(it - 1)) goto out;
+            if (!issue_pv()) goto out;
         }
-    } else if (warp < 15) {
+    } else if (warp == 21 || warp == 22) {
         // ------------------------------------------------------------ loads
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_REST));
-        const bool keys = warp == 13;
+        const bool keys = warp == 21;
         uint64_t *full = keys ? sm.rk_full : sm.rv_full, *empty = keys ? sm.rk_empty : sm.rv_empty;
         uint8_t *ring = keys ? sm.raw_k[0] : sm.raw_v[0];
         const uint8_t *codes = p.codes + (keys ? 0 : C::SIDE_BYTES);
         uint32_t it = 0;
-        for (; more; more = cursor_next(p, cur)) {
+        while (next_piece(ok)) {
             const int32_t *ids = p.table + (size_t)cur.seq * p.table_stride;
-            const int last = (int)min((long long)cur.t.row0 + TM - 1,
-                                      (long long)cur.s.nq * p.group - 1) / p.group;
-            const int hi = p.causal ? min(cur.s.len, cur.t.pos0 + last + 1) : cur.s.len;
-            const int lo = p.window
-                               ? max(0, cur.t.pos0 + cur.t.row0 / p.group - p.window + 1) : 0;
+            const int hi = cur.hi, lo = cur.lo;
             // the lookups of 32 groups (four units) at a time, the next ones ahead of their use
             int id;
             float2 sc;
             auto look = [&](int c) {
                 id = -1;
                 sc = make_float2(0.f, 0.f);
-                const int t0 = (cur.t.first + cur.c0 + c) * TN + lane * KV_GROUP;
+                const int t0 = cur.key0 + c * TN + lane * KV_GROUP;
                 if (c + lane / GROUPS < cur.n && t0 < hi && t0 + KV_GROUP > lo) {
                     id = __ldg(ids + (t0 >> p.log_block));
                     if (id < 0 || id >= p.n_blocks) {
@@ -1020,11 +1013,16 @@ __global__ void __launch_bounds__(THREADS, 1)
                                               __shfl_sync(~0u, sc_now.y, from));
                 const unsigned there = __ballot_sync(~0u, gid >= 0) & 0xFFu;
                 if (!wait(&empty[slot], it / RAW + 1)) goto out;
+                if (keys) {  // whoever sees the keys (and what follows from them) sees these
+                    if (lane < GROUPS) sm.sc[it % SC][lane] = gs;
+                    if (lane == 0) sm.valid[it % SC] = there;
+                    __syncwarp();
+                }
                 if (lane == 0)
                     mbar_arrive_tx(&full[slot], __popc(there) * C::SIDE_BYTES);
                 __syncwarp();
                 if (lane < GROUPS && gid >= 0) {
-                    const int t0 = (cur.t.first + cur.c0 + c) * TN + lane * KV_GROUP;
+                    const int t0 = cur.key0 + c * TN + lane * KV_GROUP;
                     const int grp = (t0 & ((1 << p.log_block) - 1)) / KV_GROUP;
                     const size_t bh = (size_t)gid * p.kv_heads + cur.head;
                     bulk_load(ring + (size_t)(slot * GROUPS + lane) * C::SIDE_BYTES,
@@ -1032,34 +1030,141 @@ __global__ void __launch_bounds__(THREADS, 1)
                                           (size_t)(2 * C::SIDE_BYTES),
                               C::SIDE_BYTES, &full[slot]);
                 }
-                if (keys) {
-                    if (lane < GROUPS) sm.sc[it % SC][lane] = gs;
-                    if (lane == 0) sm.valid[it % SC] = there;
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sm.sc_full[it % SC]);
-                }
             }
         }
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_REST));
+    } else if (warp == 23) {
+        // ------------------------------------------------------------ this CTA's pieces
+        // twice over the sequences, 32 at a time: the line's length; then where the part starts
+        long long total = 0, per = 0, u0 = 0, u1 = 0, at = 0, in = 0;
+        int seq = -1;
+#pragma unroll 1
+        for (int round = 0; round < 2 && seq < 0; round++) {
+            at = 0;
+#pragma unroll 1
+            for (int base = 0; base < p.n_seqs && seq < 0; base += 32) {
+                long long x = 0;
+                bool big = false;
+                if (base + lane < p.n_seqs) {
+                    const AttnSeq s = attn_seq(p, base + lane);
+                    const int tiles = tiles_of(p, s);
+                    big = tiles > 2;
+#pragma unroll 1
+                    for (int r = 0; r < tiles && !big; r++)
+                        x += tile_of(p, s, r).units + TILE_COST;
+                }
+                unsigned left = __ballot_sync(~0u, big);
+#pragma unroll 1
+                for (; left; left &= left - 1) {  // a long one: all lanes over its tiles
+                    const int i = __ffs(left) - 1;
+                    const long long y = line_of(p, attn_seq(p, base + i), 0, lane);
+                    if (lane == i) x = y;
+                }
+                x *= p.kv_heads;
+                long long upto = x;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const long long y = __shfl_up_sync(~0u, upto, d);
+                    if (lane >= d) upto += y;
+                }
+                if (round == 1) {
+                    const unsigned hit = __ballot_sync(~0u, u0 < at + upto);
+                    if (hit) {
+                        const int i = __ffs(hit) - 1;
+                        seq = base + i;
+                        in = u0 - (at + __shfl_sync(~0u, upto - x, i));
+                        at = u0 - in;
+                    }
+                }
+                if (seq < 0) at += __shfl_sync(~0u, upto, 31);
+            }
+            if (round == 0) {
+                total = at;
+                per = (total + gridDim.x - 1) / gridDim.x;
+                u0 = min(per * blockIdx.x, total);
+                u1 = min(u0 + per, total);
+                if (u0 >= u1) break;
+            }
+        }
+        // the tile within the sequence: tiles from the last, kv heads of each together
+        AttnSeq s{};
+        Tile t{};
+        int tile = 0, head = 0;
+        long long start = at;  // the line's unit where the tile (and head) starts
+        if (seq >= 0) {
+            s = attn_seq(p, seq);
+            int lo = 0, hi = tiles_of(p, s) - 1;  // the last tile whose line includes `in`
+#pragma unroll 1
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (line_of(p, s, mid, lane) * p.kv_heads > in) lo = mid;
+                else hi = mid - 1;
+            }
+            tile = lo;
+            t = tile_of(p, s, tile);
+            const int len = t.units + TILE_COST;
+            const long long before = line_of(p, s, tile + 1, lane) * p.kv_heads;
+            head = (int)((in - before) / len);
+            start = at + before + (long long)head * len;
+        }
+        for (uint32_t i = 0;;) {
+            const bool end = seq < 0 || start >= u1;
+            const long long base = start + TILE_COST;
+            const int c0 = (int)max(u0 - base, 0ll);
+            const int n = end ? 0 : (int)max(min(base + t.units, u1) - (base + c0), 0ll);
+            if (end || n) {
+                if (!wait(&sm.piece_empty[i & 1], (i >> 1) + 1)) goto out;
+                if (lane == 0) {
+                    Piece q{};
+                    if (!end) {
+                        const int first = t.pos0 + t.row0 / p.group;
+                        const int last = t.pos0 + (t.row0 + TM - 1) / p.group;
+                        q.n = n;
+                        q.key0 = (t.first + c0) * TN;
+                        q.row0 = t.row0, q.head = head, q.q0 = s.q0, q.nq = s.nq;
+                        q.pos0 = t.pos0, q.len = s.len, q.lo = t.lo, q.hi = t.hi;
+                        q.all_hi = p.causal ? min(s.len, first + 1) : s.len;
+                        q.all_lo = p.window ? last - p.window + 1 : 0;
+                        q.seq = seq;
+                        q.cta0 = (int)(base / per);
+                        q.cta1 = (int)((base + t.units - 1) / per);
+                    }
+                    sm.pieces[i & 1] = q;
+                    mbar_arrive(&sm.piece_full[i & 1]);
+                }
+                __syncwarp();
+                i++;
+            }
+            if (end) break;
+            start += TILE_COST + t.units;
+            if (++head == p.kv_heads) {
+                head = 0;
+                if (--tile < 0) {
+                    do {
+                        if (++seq == p.n_seqs) break;
+                        s = attn_seq(p, seq);
+                    } while (s.nq == 0);
+                    tile = tiles_of(p, s) - 1;
+                }
+                t = tile_of(p, s, tile);
+            }
+        }
     }
 out:
     // On expiry of a wait: the loads and MMAs in flight end (bounded) before the memory goes.
-    if (warp == 12 && lane == 0) {
+    if (warp == 20 && lane == 0) {
         tc_commit(&sm.done);
         const unsigned long long t0 = globaltimer();
         while (!mbar_try(&sm.done, 0) && globaltimer() - t0 < WAIT_NS) {
         }
     }
     __syncwarp();
-    if ((warp == 13 || warp == 14) && *abort_flag) {
+    if ((warp == 21 || warp == 22) && *abort_flag) {
         const unsigned long long t0 = globaltimer();
         while (globaltimer() - t0 < 50000000ull) __nanosleep(1000);  // 50 ms: any copy has landed
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 12)
+    if (warp == 20)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                      "r"(512));
 }
