@@ -768,12 +768,17 @@ int jkb_kv_append(jkb_kv_cache *cache, const jkb_rows *k, const jkb_rows *v,
  * taken, sequences without room. Negative lengths count as 0. New tokens past n_slots get no
  * slot (counts[0] says how many there are). */
 #define JKB_KV_MAX_SEQS 8192
-int jkb_kv_build_tables(int32_t *block_table, size_t n_seqs, size_t row_blocks,
-                        size_t table_stride, int32_t *slots, int32_t *positions, size_t n_slots,
-                        int32_t *q_starts, int32_t *kv_lens, int32_t *counts,
-                        const int32_t *ctx_lens, const int32_t *new_lens,
-                        const int32_t *free_blocks, size_t n_free, size_t block_tokens,
-                        void *stream);
+typedef struct {
+    int32_t *block_table;
+    size_t n_seqs, row_blocks, table_stride;
+    int32_t *slots, *positions;
+    size_t n_slots;
+    int32_t *q_starts, *kv_lens, *counts;
+    const int32_t *ctx_lens, *new_lens;
+    const int32_t *free_blocks;
+    size_t n_free, block_tokens;
+} jkb_kv_tables_args;
+int jkb_kv_build_tables(const jkb_kv_tables_args *args, void *stream);
 
 /* Scratch of the attention calls over caches of one head_dim: partial results where the tokens
  * of a sequence are split over the GPU. Calls that may overlap on the GPU need one each. */

@@ -712,46 +712,45 @@ int jkb_kv_append(jkb_kv_cache *c, const jkb_rows *k, const jkb_rows *v, const i
     return e == cudaSuccess ? JKB_OK : fail_cuda(e, fn);
 }
 
-int jkb_kv_build_tables(int32_t *block_table, size_t n_seqs, size_t row_blocks,
-                        size_t table_stride, int32_t *slots, int32_t *positions, size_t n_slots,
-                        int32_t *q_starts, int32_t *kv_lens, int32_t *counts,
-                        const int32_t *ctx_lens, const int32_t *new_lens,
-                        const int32_t *free_blocks, size_t n_free, size_t block_tokens,
-                        void *stream) {
+int jkb_kv_build_tables(const jkb_kv_tables_args *a, void *stream) {
     static const char *fn = "kv_build_tables";
-    const int lb = log2_block(block_tokens);
+    if (!a) return fail(JKB_E_INVALID, fn, 0, 0, 0, "null arguments");
+    const int lb = log2_block(a->block_tokens);
     if (lb < 0)
-        return fail(JKB_E_BOUNDS, fn, 0, block_tokens, 128,
-                    "block_tokens %zu is not 16, 32, 64 or 128", block_tokens);
-    if (n_seqs > JKB_KV_MAX_SEQS)
-        return fail(JKB_E_BOUNDS, fn, 0, n_seqs, JKB_KV_MAX_SEQS, "%zu sequences, at most %d",
-                    n_seqs, JKB_KV_MAX_SEQS);
-    if (row_blocks > (size_t)INT32_MAX / block_tokens || table_stride < row_blocks)
-        return fail(JKB_E_BOUNDS, fn, 0, row_blocks, table_stride,
-                    "table rows of %zu blocks, %zu apart", row_blocks, table_stride);
-    if (n_slots > (size_t)INT32_MAX - 4 || n_free > (size_t)INT32_MAX)
-        return fail(JKB_E_BOUNDS, fn, 0, n_slots, INT32_MAX, "%zu slots, %zu free blocks",
-                    n_slots, n_free);
-    if (!q_starts || !counts || (n_slots && (!slots || !positions)) || (n_free && !free_blocks) ||
-        (n_seqs && (!kv_lens || !ctx_lens || !new_lens || (row_blocks && !block_table))))
+        return fail(JKB_E_BOUNDS, fn, 0, a->block_tokens, 128,
+                    "block_tokens %zu is not 16, 32, 64 or 128", a->block_tokens);
+    if (a->n_seqs > JKB_KV_MAX_SEQS)
+        return fail(JKB_E_BOUNDS, fn, 0, a->n_seqs, JKB_KV_MAX_SEQS, "%zu sequences, at most %d",
+                    a->n_seqs, JKB_KV_MAX_SEQS);
+    if (a->row_blocks > (size_t)INT32_MAX / a->block_tokens || a->table_stride < a->row_blocks)
+        return fail(JKB_E_BOUNDS, fn, 0, a->row_blocks, a->table_stride,
+                    "table rows of %zu blocks, %zu apart", a->row_blocks, a->table_stride);
+    if (a->n_slots > (size_t)INT32_MAX - 4 || a->n_free > (size_t)INT32_MAX)
+        return fail(JKB_E_BOUNDS, fn, 0, a->n_slots, INT32_MAX, "%zu slots, %zu free blocks",
+                    a->n_slots, a->n_free);
+    if (!a->q_starts || !a->counts || (a->n_slots && (!a->slots || !a->positions)) ||
+        (a->n_free && !a->free_blocks) ||
+        (a->n_seqs &&
+         (!a->kv_lens || !a->ctx_lens || !a->new_lens || (a->row_blocks && !a->block_table))))
         return fail(JKB_E_INVALID, fn, 0, 0, 0, "null pointer");
-    const void *ptrs[] = {block_table, slots,    positions, q_starts,   kv_lens,
-                          counts,      ctx_lens, new_lens,  free_blocks};
+    const void *ptrs[] = {a->block_table, a->slots,    a->positions, a->q_starts,   a->kv_lens,
+                          a->counts,      a->ctx_lens, a->new_lens,  a->free_blocks};
     for (const void *p : ptrs)
         if (int rc = check_align(p, 4, fn, "int32")) return rc;
-    const size_t smem = (2 * n_seqs + 1) * 4;
+    const size_t smem = (2 * a->n_seqs + 1) * 4;
     if (smem > 48 * 1024) {
         cudaError_t e = cudaFuncSetAttribute(
             tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return fail_cuda(e, fn);
     }
-    const size_t want = (n_slots + 4 * TABLE_THREADS - 1) / (4 * TABLE_THREADS);
+    const size_t want = (a->n_slots + 4 * TABLE_THREADS - 1) / (4 * TABLE_THREADS);
     const size_t most = 2 * (size_t)num_sms();
     const unsigned grid = (unsigned)(want < 1 ? 1 : want > most ? most : want);
     cudaError_t e = launch_pdl(tables_kernel, dim3(grid), dim3(TABLE_THREADS), smem,
-                               as_stream(stream), block_table, (int)n_seqs, (int)row_blocks,
-                               table_stride, slots, positions, (int)n_slots, q_starts, kv_lens,
-                               counts, ctx_lens, new_lens, free_blocks, (int)n_free, lb);
+                               as_stream(stream), a->block_table, (int)a->n_seqs,
+                               (int)a->row_blocks, a->table_stride, a->slots, a->positions,
+                               (int)a->n_slots, a->q_starts, a->kv_lens, a->counts, a->ctx_lens,
+                               a->new_lens, a->free_blocks, (int)a->n_free, lb);
     return e == cudaSuccess ? JKB_OK : fail_cuda(e, fn);
 }
 

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT_DIR = os.path.dirname(PKG_DIR)
@@ -76,36 +77,12 @@ class jkb_act_q8_view(C.Structure):
     ]
 
 
-class jkb_rows(C.Structure):
-    _fields_ = [
-        ("data", C.c_void_p),
-        ("type", C.c_int32),
-        ("token_stride", C.c_size_t),
-        ("head_stride", C.c_size_t),
-    ]
-
-
-class jkb_attn_args(C.Structure):
-    _fields_ = [
-        ("cache", C.c_void_p),
-        ("ws", C.c_void_p),
-        ("q", jkb_rows),
-        ("out", jkb_rows),
-        ("lse", C.c_void_p),
-        ("n_tokens", C.c_size_t),
-        ("n_heads", C.c_size_t),
-        ("block_table", C.c_void_p),
-        ("kv_lens", C.c_void_p),
-        ("q_starts", C.c_void_p),
-        ("n_seqs", C.c_size_t),
-        ("row_blocks", C.c_size_t),
-        ("table_stride", C.c_size_t),
-        ("max_new", C.c_size_t),
-        ("window", C.c_size_t),
-        ("scale", C.c_float),
-        ("causal", C.c_int32),
-    ]
-
+# Argument structs of the calls that run many times a step are packed as bytes, which takes a
+# fraction of a ctypes structure's time. "@": the C layout.
+JKB_ROWS = "PiNN"                                     # data, type, token_stride, head_stride
+pack_rows = struct.Struct("@" + JKB_ROWS).pack
+pack_attn_args = struct.Struct("@PP" + 2 * JKB_ROWS + "PNNPPPNNNNNfi").pack
+pack_kv_tables_args = struct.Struct("@PNNNPPNPPPPPPNN").pack
 
 P, S, I, F = C.c_void_p, C.c_size_t, C.c_int, C.c_float
 PP = C.POINTER(C.c_void_p)
@@ -254,11 +231,11 @@ SIGNATURES = {
     "jkb_kv_cache_import": [P, P, S, P, P, P, P, P],
     "jkb_kv_cache_export": [P, P, S, P, P, P, P, P],
     "jkb_kv_cache_read": [P, P, S, P, P, P],
-    "jkb_kv_append": [P, C.POINTER(jkb_rows), C.POINTER(jkb_rows), P, S, P],
-    "jkb_kv_build_tables": [P, S, S, S, P, P, S, P, P, P, P, P, P, S, S, P],
+    "jkb_kv_append": [P, C.c_char_p, C.c_char_p, P, S, P],
+    "jkb_kv_build_tables": [C.c_char_p, P],
     "jkb_attn_workspace_create": [P, PP],
     "jkb_attn_workspace_destroy": [P],
-    "jkb_attention_kv8": [C.POINTER(jkb_attn_args), P],
+    "jkb_attention_kv8": [C.c_char_p, P],
 }
 _RESTYPE = {"jkb_last_error": C.c_char_p, "jkb_clear_error": None,
             "jkb_act_q8_view_scratch_bytes_for_row": C.c_size_t}

@@ -1303,29 +1303,44 @@ def repack_q4_k_m_parallel_slices(view: TensorView, rows: int, cols: int, tile_r
 
 # ------------------------------------------------------------------------------- 8-bit kv cache
 
+# These calls run many times a step, some for a few microseconds of GPU work: they look a tensor
+# over in few steps, and ask for the current stream's handle without making a Stream object.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream_of(stream, t: torch.Tensor) -> int:
+    """The stream's handle; None: the current stream of t's device."""
+    if stream is None and _raw_stream is not None:
+        return _raw_stream(t.get_device())
+    return _stream(stream)
+
+
 _ROW_TYPES = {torch.float32: int(QuantType.F32), torch.float16: int(QuantType.F16),
               torch.bfloat16: int(QuantType.BF16)}
 
 
-def _rows(t: torch.Tensor, what: str, heads: int = None, dim: int = None) -> "_lib.jkb_rows":
-    """jkb_rows of a [tokens, heads, dim] CUDA tensor whose elements of a head are adjacent."""
-    if not t.is_cuda or t.dim() != 3:
-        raise TypeError(f"{what}: expected a [tokens, heads, dim] CUDA tensor")
+def _rows(t: torch.Tensor, what: str, heads: int, dim: int):
+    """(data, type, token stride, head stride) of a [tokens, heads, dim] CUDA tensor whose elements of a head are adjacent."""
     kind = _ROW_TYPES.get(t.dtype)
-    if kind is None:
-        raise TypeError(f"{what}: {t.dtype} is none of float32, float16 and bfloat16")
-    shape, stride = t.shape, t.stride()
-    if (heads is not None and shape[1] != heads) or (dim is not None and shape[2] != dim):
-        raise ValueError(f"{what}: shape {tuple(shape)}, expected [tokens, {heads}, {dim}]")
-    if stride[2] != 1 and shape[2] > 1 or stride[0] < 0 or stride[1] < 0:
+    if kind is None or not t.is_cuda or t.dim() != 3:
+        raise TypeError(f"{what}: expected a [tokens, heads, dim] CUDA tensor of float32, float16 "
+                        f"or bfloat16, got {t.dtype} with {t.dim()} dimensions")
+    _, h, d = t.shape
+    if h != heads or d != dim:
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected [tokens, {heads}, {dim}]")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 and d > 1:
         raise ValueError(f"{what}: the elements of a head must be adjacent")
-    return _lib.jkb_rows(t.data_ptr(), kind, stride[0], stride[1])
+    return t.data_ptr(), kind, s0, s1
+
+
+_I32 = torch.int32
 
 
 def _i32(t: torch.Tensor, what: str) -> int:
-    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
-        raise TypeError(f"{what}: expected a contiguous int32 CUDA tensor")
-    return t.data_ptr()
+    if t.dtype is _I32 and t.is_cuda and t.is_contiguous():
+        return t.data_ptr()
+    raise TypeError(f"{what}: expected a contiguous int32 CUDA tensor")
 
 
 def _table(t: torch.Tensor):
@@ -1366,7 +1381,7 @@ class KvCache:
         n = blocks.numel()
         shape = (n, self.n_kv_heads, self.block_tokens, self.head_dim)
         for t in (k, v):
-            if t.dtype != dtype or tuple(t.shape) != shape:
+            if t.dtype is not dtype or t.shape != shape:
                 raise ValueError(f"expected {dtype} planes of shape {shape}, got {t.dtype} "
                                  f"{tuple(t.shape)}")
         return _i32(blocks, "blocks"), n, _dptr(k), _dptr(v)
@@ -1395,7 +1410,7 @@ class KvCache:
         """The values code * scale of the blocks, float32 [n, kv heads, block tokens, head dim]."""
         _check(_L().jkb_kv_cache_read(self.handle, *self._planes(blocks, k_out, v_out,
                                                                  torch.float32),
-                                      _stream(stream)))
+                                      _stream_of(stream, blocks)))
 
     def destroy(self):
         if getattr(self, "_h", None):
@@ -1420,7 +1435,8 @@ def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Ten
     n = slots.numel()
     if k.shape[0] != n or v.shape[0] != n:
         raise ValueError(f"{k.shape[0]} key rows and {v.shape[0]} value rows for {n} slots")
-    _check(_L().jkb_kv_append(cache.handle, kr, vr, _i32(slots, "slots"), n, _stream(stream)))
+    _check(_L().jkb_kv_append(cache.handle, _lib.pack_rows(*kr), _lib.pack_rows(*vr),
+                              _i32(slots, "slots"), n, _stream_of(stream, k)))
 
 
 def kv_build_tables(block_table, slots, positions, q_starts, kv_lens, counts, ctx_lens, new_lens,
@@ -1432,15 +1448,16 @@ def kv_build_tables(block_table, slots, positions, q_starts, kv_lens, counts, ct
     token), q_starts [sequences + 1], kv_lens [sequences] and counts [3]: new tokens, blocks
     taken, sequences without room."""
     ptr, n, width, stride = _table(block_table)
+    n_slots = slots.numel()
     if (ctx_lens.numel() != n or new_lens.numel() != n or kv_lens.numel() != n
-            or q_starts.numel() != n + 1 or counts.numel() != 3
-            or positions.numel() != slots.numel()):
+            or q_starts.numel() != n + 1 or counts.numel() != 3 or positions.numel() != n_slots):
         raise ValueError("lengths of the tables' tensors do not match")
-    _check(_L().jkb_kv_build_tables(
-        ptr, n, width, stride, _i32(slots, "slots"), _i32(positions, "positions"), slots.numel(),
+    args = _lib.pack_kv_tables_args(
+        ptr, n, width, stride, _i32(slots, "slots"), _i32(positions, "positions"), n_slots,
         _i32(q_starts, "q_starts"), _i32(kv_lens, "kv_lens"), _i32(counts, "counts"),
         _i32(ctx_lens, "ctx_lens"), _i32(new_lens, "new_lens"), _i32(free_blocks, "free_blocks"),
-        free_blocks.numel(), block_tokens, _stream(stream)))
+        free_blocks.numel(), block_tokens)
+    _check(_L().jkb_kv_build_tables(args, _stream_of(stream, block_table)))
 
 
 class AttentionWorkspace:
@@ -1478,7 +1495,9 @@ def attention_kv8(out, q, cache: KvCache, workspace: AttentionWorkspace, block_t
     are [tokens, heads, head dim] of one type, float32, float16 or bfloat16; query head h reads kv
     head h // (heads / kv heads). window > 0 hides tokens that are window or more back. A query
     that sees nothing gives 0 and lse -inf. lse: None or float32 [tokens, heads]."""
-    n, heads = q.shape[0], q.shape[1]
+    if q.dim() != 3:
+        raise TypeError("q: expected a [tokens, heads, dim] CUDA tensor")
+    n, heads, _ = q.shape
     qr = _rows(q, "q", heads, cache.head_dim)
     outr = _rows(out, "out", heads, cache.head_dim)
     if out.shape[0] != n:
@@ -1491,8 +1510,8 @@ def attention_kv8(out, q, cache: KvCache, workspace: AttentionWorkspace, block_t
     if kv_lens.numel() != seqs or q_starts.numel() != seqs + 1:
         raise ValueError(f"{kv_lens.numel()} lengths and {q_starts.numel()} starts for {seqs} "
                          "sequences")
-    args = _lib.jkb_attn_args(
-        cache.handle, workspace.handle, qr, outr, _dptr(lse), n, heads, ptr,
+    args = _lib.pack_attn_args(
+        cache.handle, workspace.handle, *qr, *outr, _dptr(lse) or 0, n, heads, ptr,
         _i32(kv_lens, "kv_lens"), _i32(q_starts, "q_starts"), seqs, width, stride, max_new,
         window, scale, 1 if causal else 0)
-    _check(_L().jkb_attention_kv8(args, _stream(stream)))
+    _check(_L().jkb_attention_kv8(args, _stream_of(stream, q)))
