@@ -15,16 +15,18 @@
 //     for its f32 lse: 1e-5 off.)
 //   * p v runs as mma.m16n8k16 on f16: p, times the block's value scale relative to a power of
 //     two, is split into two f16 (22 bits; the second in the A tile's lower half), the codes are
-//     exact in f16. The tensor core truncates its sums, so each 16-token step starts from zero
-//     and is added to o in f32 on the FMA pipe, together with the rescale.
+//     exact in f16. The tensor core truncates its sums, so each step starts from zero and is
+//     added to o in f32 on the FMA pipe, together with the rescale. (A weight below 2^-39 of its
+//     row's largest falls out of f16's range and counts as 0.)
 //
-// A group of 16 tokens (kv_cache.cuh) is one bulk copy and one step of one warp. The four warps
-// of a CTA take consecutive groups, each through its own ring of STAGES groups, and keep their
-// own (m, l, o): they meet only when a row tile's tokens end. The tokens of all sequences and kv
-// heads form one line of 64-token units, cut into equal parts, one a CTA, whatever the lengths
-// (which only the device knows): a part that holds a piece of a row tile leaves (m, l, o) in the
-// workspace, and the piece that arrives last adds all of them in the order of the line, so the
-// result does not depend on which one that is.
+// A step of one warp is G groups of 16 tokens (kv_cache.cuh), each one bulk copy into the warp's
+// ring. Two groups share a step's softmax and its o update: 300 instructions for 16 tokens of
+// 128 dims in place of 475 with one. The four warps of a CTA take consecutive steps and keep
+// their own (m, l, o): they meet only when a row tile's tokens end. The tokens of all sequences
+// and kv heads form one line of units of four steps, cut into equal parts, one a CTA, whatever
+// the lengths (which only the device knows): a part that holds a piece of a row tile leaves
+// (m, l, o) in the workspace, and the piece that arrives last adds all of them in the order of
+// the line, so the result does not depend on which one that is.
 #include "kv_attn.cuh"
 #include "ptx.cuh"
 
@@ -36,8 +38,10 @@ namespace jkb {
 
 namespace {
 
-constexpr int NW = 4;                  // warps of a CTA
-constexpr int UNIT = NW * KV_GROUP;    // tokens of a unit
+constexpr int NW = 4;        // warps of a CTA
+// CTAs an SM: 8 warps of up to 255 registers. 12 warps of 168 were 3% faster over long ragged
+// contexts and 15 to 30% slower where row tiles are short or split over many CTAs.
+constexpr int DEC_CTAS = 2;
 
 constexpr int ND = 3;                  // digits of a query element
 
@@ -46,28 +50,31 @@ struct DecCfg {
     static constexpr int DT = DT_;      // 32-element chunks of a head
     static constexpr int ROWS = ROWS_;  // 8: two digits share an MMA; 16: one each
     static constexpr int DIM = 32 * DT;
+    static constexpr int G = DT <= 4 ? 2 : 1;     // groups a step (registers and shared memory)
     static constexpr int STAGES = 3;
-    // 12 warps an SM hide the steps' latency; the 16-row tile needs the registers of 8
-    static constexpr int CTAS = DT <= 4 && ROWS == 8 ? 3 : 2;
+    static constexpr int STEP = G * KV_GROUP;     // tokens of a step
+    static constexpr int UNIT = NW * STEP;        // of a unit
+    static constexpr int BATCH = 32 / G;          // steps that are looked up together
     static constexpr int GROUP_BYTES = 32 * DIM;
-    static constexpr int PASS = DIM / 2;  // dims merged at a time
+    static constexpr int PASSES = 2;
+    static constexpr int PASS = DIM / PASSES;  // dims merged at a time
 };
 
 struct StepInfo {
-    unsigned long long src;  // the group's codes; 0: no visible token in it
-    float ks, vs;
-    int seq, item;           // item: kv head * row tiles + row tile
-    int t0;
-    int flags;               // FIRST / LAST of this CTA's piece, WHOLE row tile
+    uint32_t src[2];  // the groups' numbers in the cache, + 1; 0: no visible token in it
+    float2 sc[2];     // (ks, vs)
+    int seq, item;    // item: kv head * row tiles + row tile
+    int t0;           // first token (a multiple of 16), and the flags
 };
-enum { STEP_FIRST = 1, STEP_LAST = 2, STEP_WHOLE = 4 };
+// FIRST / LAST step of this CTA's piece of a row tile, the piece is the WHOLE tile
+enum { STEP_FIRST = 1, STEP_LAST = 2, STEP_WHOLE = 4, STEP_FLAGS = 15 };
 
 template <class C>
 struct DecSmem {
-    alignas(128) uint8_t ring[NW][C::STAGES][C::GROUP_BYTES];
+    alignas(128) uint8_t ring[NW][C::STAGES][C::G * C::GROUP_BYTES];
     alignas(16) float merge[NW][C::ROWS][C::PASS + 4];
     float row_m[NW][C::ROWS], row_l[NW][C::ROWS];
-    StepInfo info[NW][64];  // two batches of 32 steps
+    StepInfo info[NW][2 * C::BATCH];
     uint64_t full[NW][C::STAGES];
     long long warp_sum[NW];
     int abort_flag, is_last;
@@ -75,31 +82,36 @@ struct DecSmem {
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                        uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
         "{%0,%1,%2,%3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// c = a b (FIRST) or c += a b
+template <bool FIRST>
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if (FIRST)
+        asm(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint64_t pkf(float a, float b) {
+    return pk2(__float_as_uint(a), __float_as_uint(b));
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-__device__ __forceinline__ void bulk_load(void *dst, unsigned long long src, uint32_t bytes,
-                                          uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-        ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
-        : "memory");
 }
 // Value bytes (code + 128) of tokens 2t, 2t + 1 (lo) and 2t + 8, 2t + 9 (hi) as f16 codes:
 // 0x6400 | byte is 1024 + byte.
@@ -187,25 +199,27 @@ __device__ __forceinline__ void store4(const AttnParams &p, int type, size_t i, 
     }
 }
 
-// A query row is held as integers |n| <= MOST in ND signed base-256 digits: x = unit * n. A row
-// with a non-finite element has unit NaN, so that its output is NaN; below 1e-30 the row counts
-// as 0 (its scores are 0 to f32's accuracy).
-constexpr float MOST = 8355711.0f;  // 127 * (65536 + 256 + 1)
+// A query row is held as integers |n| < 127 * (65536 + 256 + 1) in three signed base-256 digits,
+// x = unit * n: the bytes of (n + 0x808080) ^ 0x808080. MOST leaves room for the rounding of
+// x / unit. A row with a non-finite element has unit NaN, so that its output is NaN; below 1e-30
+// the row counts as 0 (its scores are 0 to f32's accuracy).
+constexpr float MOST = 8355700.0f;
 
 // Units of one sequence and its row tiles.
-template <int ROWS>
+template <class C>
 __device__ __forceinline__ void seq_units(const AttnParams &p, const AttnSeq &s, int &tiles,
                                           int &first_unit, int &units) {
-    tiles = (int)(((long long)s.nq * p.group + ROWS - 1) / ROWS);
-    first_unit = s.lo / UNIT;
-    units = max(1, (s.len + UNIT - 1) / UNIT - first_unit);
+    tiles = (int)(((long long)s.nq * p.group + C::ROWS - 1) / C::ROWS);
+    first_unit = s.lo / C::UNIT;
+    units = max(1, (s.len + C::UNIT - 1) / C::UNIT - first_unit);
 }
 
 template <class C>
-__global__ void __launch_bounds__(32 * NW, C::CTAS)
+__global__ void __launch_bounds__(32 * NW, DEC_CTAS)
     attn_decode_kernel(const __grid_constant__ AttnParams p, const int type) {
     constexpr int ROWS = C::ROWS, DT = C::DT, DIM = C::DIM, STAGES = C::STAGES;
     constexpr int RH = ROWS / 8;  // rows of a thread
+    constexpr int G = C::G, BATCH = C::BATCH;
     extern __shared__ uint8_t smem_raw[];
     DecSmem<C> &sm =
         *reinterpret_cast<DecSmem<C> *>((((uintptr_t)smem_raw) + 127) & ~(uintptr_t)127);
@@ -226,7 +240,7 @@ __global__ void __launch_bounds__(32 * NW, C::CTAS)
         long long sum = 0;
         for (int i = a; i < b; i++) {
             int tiles, first, units;
-            seq_units<ROWS>(p, attn_seq(p, i), tiles, first, units);
+            seq_units<C>(p, attn_seq(p, i), tiles, first, units);
             sum += (long long)p.kv_heads * tiles * units;
         }
         long long inc = sum;
@@ -240,7 +254,7 @@ __global__ void __launch_bounds__(32 * NW, C::CTAS)
         for (int w = 0; w < warp; w++) at += sm.warp_sum[w];
         for (int i = a; i < b; i++) {
             int tiles, first, units;
-            seq_units<ROWS>(p, attn_seq(p, i), tiles, first, units);
+            seq_units<C>(p, attn_seq(p, i), tiles, first, units);
             prefix[i] = at;
             at += (long long)p.kv_heads * tiles * units;
         }
@@ -253,83 +267,142 @@ __global__ void __launch_bounds__(32 * NW, C::CTAS)
     const int steps = (int)min(u1 - u0, (long long)INT32_MAX);
     if (steps == 0) return;
 
-    // Fills info[] for steps base .. base + 31 (lane i: step base + i), a multiple of 32: the table
-    // entries and scales of 32 steps are fetched together, before the ring needs them.
-    auto decode = [&](int base) {
-        __syncwarp();
-        StepInfo &f = sm.info[warp][(base + lane) & 63];
-        f.src = 0;
-        f.flags = 0;
-        const long long u = u0 + base + lane;
-        if (u < u1) {
-            int a = 0, b = p.n_seqs - 1;  // the last sequence that starts at or before u
-            while (a < b) {
-                const int mid = (a + b + 1) >> 1;
-                if (prefix[mid] <= u) a = mid;
-                else b = mid - 1;
-            }
-            const AttnSeq s = attn_seq(p, a);
-            int tiles, first, units;
-            seq_units<ROWS>(p, s, tiles, first, units);
-            const long long local = u - prefix[a];
-            const int item = (int)(local / units), c = (int)(local - (long long)item * units);
-            const int head = item / tiles;
-            f.seq = a;
-            f.item = item;
-            f.t0 = (first + c) * UNIT + warp * KV_GROUP;
-            f.flags = (c == 0 || u == u0 ? STEP_FIRST : 0) |
-                      (c == units - 1 || u == u1 - 1 ? STEP_LAST : 0);
-            const long long start = u - c;
-            if (start >= u0 && start + units <= u1) f.flags |= STEP_WHOLE;
-            if (f.t0 < s.len && f.t0 + KV_GROUP > s.lo) {
-                const int id = __ldg(p.table + (size_t)a * p.table_stride +
-                                     (f.t0 >> p.log_block));
-                if (id >= 0 && id < p.n_blocks) {
-                    const size_t bh = (size_t)id * p.kv_heads + head;
-                    const float2 sc = __ldg(p.scales + bh);
-                    const int grp = (f.t0 & ((1 << p.log_block) - 1)) / KV_GROUP;
-                    f.ks = sc.x;
-                    f.vs = sc.y;
-                    f.src = (unsigned long long)(p.codes +
-                                                 ((bh << p.log_block) / KV_GROUP + grp) *
-                                                     (size_t)C::GROUP_BYTES);
-                } else {
-                    atomicOr(p.err, ERR_KV_RANGE);
-                }
-            }
-        }
-        __syncwarp();
+    // Starts the copies of a step (lane 0, by predicate: a branch would cost the warp its turn)
+    auto issue = [&](int s, const uint32_t (&src)[2]) {
+        const int n = (src[0] != 0) + (G > 1 && src[1] != 0);
+        const uint32_t bar = smem_u32(&sm.full[warp][s % STAGES]);
+        const uint32_t dst = smem_u32(sm.ring[warp][s % STAGES]);
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t"
+            "@p mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+            "r"(n * C::GROUP_BYTES), "r"((uint32_t)(lane == 0 && n))
+            : "memory");
+#pragma unroll
+        for (int i = 0; i < G; i++)
+            asm volatile(
+                "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                "@p cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes "
+                "[%0], [%1], %2, [%3];\n\t}" ::"r"(dst + i * C::GROUP_BYTES),
+                "l"(p.codes + (size_t)(src[i] - 1) * C::GROUP_BYTES), "r"(C::GROUP_BYTES),
+                "r"(bar), "r"((uint32_t)(lane == 0 && src[i]))
+                : "memory");
     };
-    int issued = 0;
-    auto issue = [&](int upto) {  // starts the copies of the steps below min(upto, steps)
-        for (; issued < min(upto, steps); issued++) {
-            if (lane == 0) {
-                const unsigned long long src = sm.info[warp][issued & 63].src;
-                if (src) {
-                    uint64_t *bar = &sm.full[warp][issued % STAGES];
-                    mbar_arrive_tx(bar, C::GROUP_BYTES);
-                    bulk_load(sm.ring[warp][issued % STAGES], src, C::GROUP_BYTES, bar);
-                }
+    // Lookups of BATCH steps at a time (lane i: group i % G of step base + i / G), each in three
+    // stages several steps apart, since each waits for a load of the one before, microseconds
+    // where the memory is busy: which token, and its table entry; its place and scales; the
+    // step's entry in info[].
+    struct Look {
+        int id, at;      // block id, token
+        int head;        // kv head; -1: no visible token
+        int seq, item, t0;
+    };
+    auto find = [&](int base) {
+        Look f;
+        f.id = f.head = -1;
+        f.at = f.seq = f.item = f.t0 = 0;
+        const long long u = u0 + base + lane / G;
+        if (u >= u1) return f;
+        int a = 0, b = p.n_seqs - 1;  // the last sequence that starts at or before u
+        while (a < b) {
+            const int mid = (a + b + 1) >> 1;
+            if (prefix[mid] <= u) a = mid;
+            else b = mid - 1;
+        }
+        const AttnSeq s = attn_seq(p, a);
+        int tiles, first, units;
+        seq_units<C>(p, s, tiles, first, units);
+        const long long local = u - prefix[a];
+        f.seq = a;
+        f.item = (int)(local / units);
+        f.head = f.item / tiles;
+        const int c = (int)(local - (long long)f.item * units);
+        const long long start = u - c;
+        f.t0 = (first + c) * C::UNIT + warp * C::STEP;
+        f.at = f.t0 + lane % G * KV_GROUP;
+        f.t0 |= (c == 0 || u == u0 ? STEP_FIRST : 0) |
+                (c == units - 1 || u == u1 - 1 ? STEP_LAST : 0) |
+                (start >= u0 && start + units <= u1 ? STEP_WHOLE : 0);
+        // the query rows of a piece that starts here, on their way to the L1
+        if (f.t0 & STEP_FIRST && warp == 0 && lane % G == 0) {
+            const int rows = min(ROWS, s.nq * p.group - (f.item - f.head * tiles) * ROWS);
+            for (int r = 0; r < rows; r++) {
+                const int row = (f.item - f.head * tiles) * ROWS + r, tok = row / p.group;
+                const size_t bytes = type == JKB_F32 ? 4 : 2;
+                const char *q = (const char *)p.q +
+                                ((size_t)(s.q0 + tok) * p.q_token +
+                                 (size_t)(f.head * p.group + row - tok * p.group) * p.q_head) *
+                                    bytes;
+                for (size_t d = 0; d < p.dim * bytes; d += 128)
+                    asm volatile("prefetch.global.L1 [%0];" ::"l"(q + d));
             }
         }
+        if (f.at < s.len && f.at + KV_GROUP > s.lo)
+            f.id = __ldg(p.table + (size_t)a * p.table_stride + (f.at >> p.log_block));
+        else
+            f.head = -1;
+        return f;
+    };
+    auto place = [&](const Look &f, float2 &sc) {  // the group's number in the cache, + 1; 0: none
+        sc = make_float2(0.f, 0.f);
+        if (f.head < 0) return 0u;
+        if (f.id < 0 || f.id >= p.n_blocks) {
+            atomicOr(p.err, ERR_KV_RANGE);
+            return 0u;
+        }
+        const size_t bh = (size_t)f.id * p.kv_heads + f.head;
+        sc = __ldg(p.scales + bh);
+        return (uint32_t)(((bh << p.log_block) | (f.at & ((1 << p.log_block) - 1))) / KV_GROUP) +
+               1;
+    };
+    auto enter = [&](int base, const Look &f, uint32_t src, float2 sc) {
+        __syncwarp();
+        StepInfo &i = sm.info[warp][(base + lane / G) % (2 * BATCH)];
+        i.src[lane % G] = src;
+        i.sc[lane % G] = sc;
+        if (lane % G == 0) {
+            i.seq = f.seq;
+            i.item = f.item;
+            i.t0 = f.t0;
+        }
+        __syncwarp();
     };
 
     // ---- running state of the current row tile ----
     uint32_t qa[ND][DT][2 * RH];  // A registers of each digit
     float m[RH], l[RH], unit[RH];
-    int lo[RH], hi[RH];
-    float o[RH][DT][8];  // dims 32 c + 8 tg + i of row g (+ 8)
+    int lo[RH], hi[RH], all_lo = 0, all_hi = 0;  // tokens that the rows see; that all see
+    uint64_t o[RH][DT][4];  // pairs: dims 32 c + 8 tg + j and + 4 + j of row g (+ 8)
     int vexp = 0;
     bool seen = false, dead = false;
     uint32_t phases = 0;
 
-    decode(0);
-    issue(STAGES);
+    Look look = find(0);
+    float2 look_sc;
+    uint32_t look_src = place(look, look_sc);
+    {   // the first copies start before their scales are there
+        uint32_t src[2] = {0, 0};
+#pragma unroll
+        for (int k = 0; k < STAGES; k++) {
+#pragma unroll
+            for (int i = 0; i < G; i++) src[i] = __shfl_sync(~0u, look_src, G * k + i);
+            if (k < steps) issue(k, src);
+        }
+    }
+    enter(0, look, look_src, look_sc);
     for (int s = 0; s < steps; s++) {
-        if ((s & 31) == 24 && s + 8 < steps) decode(s + 8);
-        const StepInfo f = sm.info[warp][s & 63];
+        const int phase = s % BATCH;
+        if (phase == 0) look = find(s + BATCH);
+        if (phase == BATCH / 2 - 2) look_src = place(look, look_sc);
+        if (phase == BATCH - STAGES - 1) enter(s - phase + BATCH, look, look_src, look_sc);
+        StepInfo f = sm.info[warp][s % (2 * BATCH)];
+        const int flags = f.t0 & STEP_FLAGS;
+        f.t0 &= ~STEP_FLAGS;
+        const bool any = f.src[0] || (G > 1 && f.src[1]);
+        // (past the last step nothing is looked up, and nothing copied)
+        const uint32_t next_src[2] = {sm.info[warp][(s + STAGES) % (2 * BATCH)].src[0],
+                                      sm.info[warp][(s + STAGES) % (2 * BATCH)].src[G - 1]};
 
-        if (f.flags & STEP_FIRST) {
+        if (flags & STEP_FIRST) {
             const AttnSeq q = attn_seq(p, f.seq);
             const int tiles = (int)(((long long)q.nq * p.group + ROWS - 1) / ROWS);
             const int head = f.item / tiles, tile = f.item - head * tiles;
@@ -348,12 +421,14 @@ __global__ void __launch_bounds__(32 * NW, C::CTAS)
 #pragma unroll
                     for (int i = 0; i < 8; i++) x[c][i] = 0.0f;
                     if (on && d < p.dim) load8(p, type, at + d, x[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < DT; c++)
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         finite &= isfinite(x[c][i]);
                         top = fmaxf(top, fabsf(x[c][i]));
                     }
-                }
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
                 const unsigned all = __ballot_sync(~0u, finite);
@@ -361,25 +436,23 @@ __global__ void __launch_bounds__(32 * NW, C::CTAS)
                 const float inv = finite && top > 1e-30f ? __fdividef(MOST, top) : 0.0f;
                 unit[r] = (finite ? top / MOST : __int_as_float(0x7FC00000)) * p.scale2;
 #pragma unroll
-                for (int c = 0; c < DT; c++) {
-                    uint32_t dg[ND][2] = {};
+                for (int c = 0; c < DT; c++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float y = finite ? x[c][i] * inv : 0.0f;
-                        int n = __float2int_rn(fminf(fmaxf(y, -MOST), MOST));
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t w[4];
 #pragma unroll
-                        for (int k = ND - 1; k >= 0; k--) {
-                            const int low = (int)(int8_t)(n & 255);
-                            dg[k][i >> 2] |= (uint32_t)(low & 255) << (8 * (i & 3));
-                            n = (n - low) >> 8;
+                        for (int i = 0; i < 4; i++) {
+                            const float y = finite ? x[c][4 * h + i] * inv : 0.0f;
+                            w[i] = (uint32_t)(__float2int_rn(y) + 0x808080) ^ 0x808080u;
                         }
+                        const uint32_t a = __byte_perm(w[0], w[1], 0x5140);
+                        const uint32_t b = __byte_perm(w[2], w[3], 0x5140);
+                        qa[2][c][2 * r + h] = __byte_perm(a, b, 0x5410);
+                        qa[1][c][2 * r + h] = __byte_perm(a, b, 0x7632);
+                        qa[0][c][2 * r + h] =
+                            __byte_perm(__byte_perm(w[0], w[1], 0x0062),
+                                        __byte_perm(w[2], w[3], 0x0062), 0x5410);
                     }
-#pragma unroll
-                    for (int k = 0; k < ND; k++) {
-                        qa[k][c][2 * r] = dg[k][0];
-                        qa[k][c][2 * r + 1] = dg[k][1];
-                    }
-                }
                 const int pos = q.len - q.nq + tok;
                 hi[r] = !on ? 0 : p.causal ? min(q.len, pos + 1) : q.len;
                 lo[r] = p.window ? max(0, pos - p.window + 1) : 0;
@@ -388,125 +461,190 @@ __global__ void __launch_bounds__(32 * NW, C::CTAS)
 #pragma unroll
                 for (int c = 0; c < DT; c++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) o[r][c][i] = 0.0f;
+                    for (int i = 0; i < 4; i++) o[r][c][i] = 0;
             }
             seen = false;
+            const int last = min((tile + 1) * ROWS, q.nq * p.group) - 1;  // of the tile's rows
+            const int pos_a = q.len - q.nq + tile * ROWS / p.group;
+            const int pos_b = q.len - q.nq + last / p.group;
+            all_hi = p.causal ? min(q.len, pos_a + 1) : q.len;
+            all_lo = p.window ? pos_b - p.window + 1 : 0;
         }
 
-        if (f.src) {
+        if (any) {
             const int st = s % STAGES;
             if (!dead && !mbar_wait(&sm.full[warp][st], (phases >> st) & 1, &sm.abort_flag, p.err,
                                     ERR_ATTN_WAIT))
                 dead = true;
             phases ^= 1u << st;
         }
-        if (f.src && !dead) {
+        if (any && !dead) {
             const uint8_t *stage = sm.ring[warp][s % STAGES];
-            // ---- scores: tokens t0 + 8 nt + 2 tg + e of rows g (+ 8) ----
-            float sc[RH][4];
+            // ---- scores: tokens t0 + 16 i + 8 nt + 2 tg + e of rows g (+ 8) ----
+            // (chunks of dims outside, so that an MMA's accumulator comes up again only after
+            // those of the other tokens and digits)
+            float sc[RH][4 * G];
+            int acc[G][2][ND][4] = {};
 #pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-                int acc[ND][4] = {};
+            for (int c = 0; c < DT; c++)
 #pragma unroll
-                for (int c = 0; c < DT; c++) {
-                    const uint2 b = *reinterpret_cast<const uint2 *>(stage + nt * 8 * DIM +
-                                                                     c * 256 + lane * 8);
-                    if (RH == 1) {
-                        mma_s8(acc[0], qa[0][c][0], qa[1][c][0], qa[0][c][1], qa[1][c][1], b.x,
-                               b.y);
-                        mma_s8(acc[2], qa[2][c][0], 0u, qa[2][c][1], 0u, b.x, b.y);
-                    } else {
+                for (int i = 0; i < G; i++)
 #pragma unroll
-                        for (int k = 0; k < ND; k++)
-                            mma_s8(acc[k], qa[k][c][0], qa[k][c][2 * RH - 2], qa[k][c][1],
-                                   qa[k][c][2 * RH - 1], b.x, b.y);
+                    for (int nt = 0; nt < 2; nt++) {
+                        const uint2 b = *reinterpret_cast<const uint2 *>(
+                            stage + i * C::GROUP_BYTES + nt * 8 * DIM + c * 256 + lane * 8);
+                        if (RH == 1) {
+                            mma_s8(acc[i][nt][0], qa[0][c][0], qa[1][c][0], qa[0][c][1],
+                                   qa[1][c][1], b.x, b.y);
+                            mma_s8(acc[i][nt][2], qa[2][c][0], 0u, qa[2][c][1], 0u, b.x, b.y);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < ND; k++)
+                                mma_s8(acc[i][nt][k], qa[k][c][0], qa[k][c][2 * RH - 2],
+                                       qa[k][c][1], qa[k][c][2 * RH - 1], b.x, b.y);
+                        }
+                    }
+#pragma unroll
+            for (int r = 0; r < RH; r++)
+#pragma unroll
+                for (int i = 0; i < G; i++) {
+                    const float f_row = unit[r] * f.sc[i].x;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int(&a)[ND][4] = acc[i][k / 2];
+                        const int e = k % 2;
+                        const int d0 = RH == 1 ? a[0][e] : a[0][2 * r + e];
+                        const int d1 = RH == 1 ? a[0][2 + e] : a[1][2 * r + e];
+                        const int d2 = RH == 1 ? a[2][e] : a[2][2 * r + e];
+                        sc[r][4 * i + k] =
+                            fmaf((float)d0, 65536.0f, fmaf((float)d1, 256.0f, (float)d2)) * f_row;
                     }
                 }
+            if (f.t0 < all_lo || f.t0 + C::STEP > all_hi || (G > 1 && !(f.src[0] && f.src[1]))) {
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
+                for (int r = 0; r < RH; r++)
 #pragma unroll
-                    for (int r = 0; r < RH; r++) {
-                        const int d0 = RH == 1 ? acc[0][e] : acc[0][2 * r + e];
-                        const int d1 = RH == 1 ? acc[0][2 + e] : acc[1][2 * r + e];
-                        const int d2 = RH == 1 ? acc[2][e] : acc[2][2 * r + e];
-                        const float v =
-                            fmaf((float)d0, 65536.0f, fmaf((float)d1, 256.0f, (float)d2));
-                        const int t = f.t0 + 8 * nt + 2 * tg + e;
-                        sc[r][2 * nt + e] =
-                            t >= lo[r] && t < hi[r] ? v * (unit[r] * f.ks) : -INFINITY;
+                    for (int k = 0; k < 4 * G; k++) {
+                        const int t = f.t0 + 16 * (k / 4) + 8 * (k / 2 % 2) + 2 * tg + k % 2;
+                        if (t < lo[r] || t >= hi[r] || !f.src[k / 4]) sc[r][k] = -INFINITY;
                     }
-                }
             }
-            // ---- the block's value scale relative to a power of two ----
-            const uint32_t vbits = __float_as_uint(f.vs);
-            const int e = (int)((vbits >> 23) & 255) - 126;
-            const float mant = (vbits & 0x7F800000u)
-                                   ? __uint_as_float((vbits & 0x807FFFFFu) | 0x3F000000u)
-                                   : 0.0f;  // vs = mant * 2^e
-            float shift = 1.0f;
+            // ---- the blocks' value scales relative to a power of two: vs = mant * 2^e ----
+            float vmul[G], shift = 1.0f;
+            int e[G], most = INT_MIN;
+#pragma unroll
+            for (int i = 0; i < G; i++) {
+                const uint32_t vb = __float_as_uint(f.sc[i].y);
+                e[i] = (int)((vb >> 23) & 255) - 126;
+                vmul[i] = (vb & 0x7F800000u) ? __uint_as_float((vb & 0x807FFFFFu) | 0x3F000000u)
+                                             : 0.0f;
+                if (f.src[i]) most = max(most, e[i]);
+            }
             if (!seen) {
-                vexp = e;
+                vexp = most;
                 seen = true;
-            } else if (e > vexp) {
-                shift = ex2((float)(vexp - e));
-                vexp = e;
+            } else if (most > vexp) {
+                shift = ex2((float)(vexp - most));
+                vexp = most;
             }
-            const float vmul = mant * ex2((float)(e - vexp + 14));
+#pragma unroll
+            for (int i = 0; i < G; i++)
+                vmul[i] = f.src[i] ? vmul[i] * ex2((float)(e[i] - vexp + 14)) : 0.0f;
             // ---- softmax step ----
-            uint32_t ph[RH][2], pl[RH][2];
-            float alpha[RH];
+            uint32_t ph[RH][G][2], pl[RH][G][2];
+            uint64_t alpha[RH];
 #pragma unroll
             for (int r = 0; r < RH; r++) {
                 float top = fmaxf(fmaxf(sc[r][0], sc[r][1]), fmaxf(sc[r][2], sc[r][3]));
+#pragma unroll
+                for (int k = 4; k < 4 * G; k++) top = fmaxf(top, sc[r][k]);
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
                 const float mn = fmaxf(m[r], top);
                 const float ref = mn == -INFINITY ? 0.0f : mn;
-                alpha[r] = ex2(m[r] - ref);
+                const float a = ex2(m[r] - ref);
                 m[r] = mn;
-                float w[4];
+                float sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = ex2(sc[r][i] - ref);
-                l[r] = fmaf(l[r], alpha[r], (w[0] + w[1]) + (w[2] + w[3]));
-                alpha[r] *= shift;
-                split_f16(w[0] * vmul, w[1] * vmul, ph[r][0], pl[r][0]);
-                split_f16(w[2] * vmul, w[3] * vmul, ph[r][1], pl[r][1]);
+                for (int i = 0; i < G; i++) {
+                    float w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) w[k] = ex2(sc[r][4 * i + k] - ref);
+                    sum += (w[0] + w[1]) + (w[2] + w[3]);
+                    split_f16(w[0] * vmul[i], w[1] * vmul[i], ph[r][i][0], pl[r][i][0]);
+                    split_f16(w[2] * vmul[i], w[3] * vmul[i], ph[r][i][1], pl[r][i][1]);
+                }
+                l[r] = fmaf(l[r], a, sum);
+                alpha[r] = pkf(a * shift, a * shift);
             }
             // ---- o = o * alpha + p v ----
 #pragma unroll
             for (int c = 0; c < DT; c++) {
-                const uint4 v4 = *reinterpret_cast<const uint4 *>(
-                    stage + 16 * DIM + c * 512 + (tg * 8 + (g ^ (2 * tg))) * 16);
-                const uint32_t vw[4] = {v4.x, v4.y, v4.z, v4.w};
+                uint32_t vw[G][4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    uint32_t b0, b1;
-                    value_f16(vw[j], b0, b1);
-                    float d[4] = {0.f, 0.f, 0.f, 0.f};
-                    if (RH == 1) {  // rows g: high parts, rows g + 8: low parts
-                        mma_f16(d, ph[0][0], pl[0][0], ph[0][1], pl[0][1], b0, b1);
-                        o[0][c][j] = fmaf(o[0][c][j], alpha[0], d[0] + d[2]);
-                        o[0][c][4 + j] = fmaf(o[0][c][4 + j], alpha[0], d[1] + d[3]);
-                    } else {
-                        mma_f16(d, pl[0][0], pl[RH - 1][0], pl[0][1], pl[RH - 1][1], b0, b1);
-                        mma_f16(d, ph[0][0], ph[RH - 1][0], ph[0][1], ph[RH - 1][1], b0, b1);
+                for (int i = 0; i < G; i++) {
+                    const uint4 v4 = *reinterpret_cast<const uint4 *>(
+                        stage + i * C::GROUP_BYTES + 16 * DIM + c * 512 +
+                        (tg * 8 + (g ^ (2 * tg))) * 16);
+                    vw[i][0] = v4.x, vw[i][1] = v4.y, vw[i][2] = v4.z, vw[i][3] = v4.w;
+                }
+                uint32_t b[G][4][2];
 #pragma unroll
-                        for (int r = 0; r < RH; r++) {
-                            o[r][c][j] = fmaf(o[r][c][j], alpha[r], d[2 * r]);
-                            o[r][c][4 + j] = fmaf(o[r][c][4 + j], alpha[r], d[2 * r + 1]);
+                for (int i = 0; i < G; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) value_f16(vw[i][j], b[i][j][0], b[i][j][1]);
+                float d[4][4];
+                if (RH == 1) {  // rows g: high parts, rows g + 8: low parts
+#pragma unroll
+                    for (int i = 0; i < G; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            if (i == 0)
+                                mma_f16<true>(d[j], ph[0][i][0], pl[0][i][0], ph[0][i][1],
+                                              pl[0][i][1], b[i][j][0], b[i][j][1]);
+                            else
+                                mma_f16<false>(d[j], ph[0][i][0], pl[0][i][0], ph[0][i][1],
+                                               pl[0][i][1], b[i][j][0], b[i][j][1]);
                         }
-                    }
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        o[0][c][j] = fma2(o[0][c][j], alpha[0],
+                                          add2(pkf(d[j][0], d[j][1]), pkf(d[j][2], d[j][3])));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < G; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            if (i == 0)
+                                mma_f16<true>(d[j], pl[0][i][0], pl[RH - 1][i][0], pl[0][i][1],
+                                              pl[RH - 1][i][1], b[i][j][0], b[i][j][1]);
+                            else
+                                mma_f16<false>(d[j], pl[0][i][0], pl[RH - 1][i][0], pl[0][i][1],
+                                               pl[RH - 1][i][1], b[i][j][0], b[i][j][1]);
+                        }
+#pragma unroll
+                    for (int i = 0; i < G; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            mma_f16<false>(d[j], ph[0][i][0], ph[RH - 1][i][0], ph[0][i][1],
+                                           ph[RH - 1][i][1], b[i][j][0], b[i][j][1]);
+#pragma unroll
+                    for (int r = 0; r < RH; r++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            o[r][c][j] =
+                                fma2(o[r][c][j], alpha[r], pkf(d[j][2 * r], d[j][2 * r + 1]));
                 }
             }
         }
         __syncwarp();
-        issue(s + 1 + STAGES);
+        if (s + STAGES < steps) issue(s + STAGES, next_src);
 
-        if (!(f.flags & STEP_LAST)) continue;
+        if (!(flags & STEP_LAST)) continue;
         // ---- the piece ends: the warps' (m, l, o) into one ----
         const AttnSeq q = attn_seq(p, f.seq);
         int tiles, first, units;
-        seq_units<ROWS>(p, q, tiles, first, units);
+        seq_units<C>(p, q, tiles, first, units);
         const int head = f.item / tiles, tile = f.item - head * tiles;
 #pragma unroll
         for (int r = 0; r < RH; r++) {
@@ -528,7 +666,7 @@ __global__ void __launch_bounds__(32 * NW, C::CTAS)
             mul[r] = ex2(m[r] - (top == -INFINITY ? 0.0f : top));
         }
         // where this piece's sums go: the output, or its slot in the workspace
-        const bool whole = f.flags & STEP_WHOLE;
+        const bool whole = flags & STEP_WHOLE;
         const long long start = prefix[f.seq] + (long long)f.item * units;
         const int cta0 = (int)(start / per), cta1 = (int)((start + units - 1) / per);
         auto slot_of = [&](int cta) {
@@ -548,7 +686,7 @@ __global__ void __launch_bounds__(32 * NW, C::CTAS)
                     (top + log2f(sum)) * 0.69314718055994531f;
         };
 #pragma unroll
-        for (int pass = 0; pass < 2; pass++) {
+        for (int pass = 0; pass < C::PASSES; pass++) {
 #pragma unroll
             for (int c = 0; c < DT; c++) {
 #pragma unroll
@@ -557,11 +695,14 @@ __global__ void __launch_bounds__(32 * NW, C::CTAS)
                     for (int k = 0; k < 2; k++) {
                         const int d = 32 * c + 8 * tg + 4 * k - pass * C::PASS;
                         if (d >= 0 && d < C::PASS) {
-                            float4 v;
-                            v.x = o[r][c][4 * k] * mul[r] * pow2;
-                            v.y = o[r][c][4 * k + 1] * mul[r] * pow2;
-                            v.z = o[r][c][4 * k + 2] * mul[r] * pow2;
-                            v.w = o[r][c][4 * k + 3] * mul[r] * pow2;
+                            float x[4];
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                float u, w;
+                                upk2(o[r][c][j], u, w);
+                                x[j] = (k ? w : u) * mul[r] * pow2;
+                            }
+                            const float4 v = make_float4(x[0], x[1], x[2], x[3]);
                             *reinterpret_cast<float4 *>(&sm.merge[warp][g + 8 * r][d]) = v;
                         }
                     }
@@ -606,23 +747,40 @@ __global__ void __launch_bounds__(32 * NW, C::CTAS)
         __threadfence();
         for (int i = tid; i < ROWS * DIM / 4; i += 32 * NW) {
             const int row = i / (DIM / 4), d = 4 * (i - row * (DIM / 4));
-            float top = -INFINITY;
-#pragma unroll 8
-            for (int c = cta0; c <= cta1; c++)
-                top = fmaxf(top, __ldcg(slot_of(c) + ROWS * DIM + row));
-            const float ref = top == -INFINITY ? 0.0f : top;
+            // one pass, the loads of NC pieces in flight together (20 were no faster over 38 pieces and
+            // slower over a few)
+            constexpr int NC = 8;
+            float top = -INFINITY, sum = 0.0f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            float sum = 0.0f;
-#pragma unroll 8
-            for (int c = cta0; c <= cta1; c++) {
-                const float *slot = slot_of(c);
-                const float w = ex2(__ldcg(slot + ROWS * DIM + row) - ref);
-                const float4 x = __ldcg(reinterpret_cast<const float4 *>(slot + row * DIM + d));
-                sum = fmaf(w, __ldcg(slot + ROWS * DIM + ROWS + row), sum);
-                v.x = fmaf(w, x.x, v.x);
-                v.y = fmaf(w, x.y, v.y);
-                v.z = fmaf(w, x.z, v.z);
-                v.w = fmaf(w, x.w, v.w);
+#pragma unroll 1
+            for (int c0 = cta0; c0 <= cta1; c0 += NC) {
+                float m_in[NC], l_in[NC];
+                float4 v_in[NC];
+#pragma unroll
+                for (int k = 0; k < NC; k++) {
+                    const float *slot = slot_of(min(c0 + k, cta1));
+                    m_in[k] = __ldcg(slot + ROWS * DIM + row);
+                    l_in[k] = __ldcg(slot + ROWS * DIM + ROWS + row);
+                    v_in[k] = __ldcg(reinterpret_cast<const float4 *>(slot + row * DIM + d));
+                }
+                float mn = top;
+#pragma unroll
+                for (int k = 0; k < NC; k++) mn = fmaxf(mn, m_in[k]);
+                const float ref = mn == -INFINITY ? 0.0f : mn;
+                const float a = ex2(top - ref);
+                top = mn;
+                sum *= a;
+                v.x *= a, v.y *= a, v.z *= a, v.w *= a;
+#pragma unroll
+                for (int k = 0; k < NC; k++) {
+                    if (c0 + k > cta1) continue;
+                    const float w = ex2(m_in[k] - ref);
+                    sum = fmaf(w, l_in[k], sum);
+                    v.x = fmaf(w, v_in[k].x, v.x);
+                    v.y = fmaf(w, v_in[k].y, v.y);
+                    v.z = fmaf(w, v_in[k].z, v.z);
+                    v.w = fmaf(w, v_in[k].w, v.w);
+                }
             }
             finish(row, d, v, top, sum);
         }
@@ -654,7 +812,7 @@ int launch_cfg(const AttnParams &p, int type, cudaStream_t st) {
         allowed = smem;
         allowed_dev = dev;
     }
-    cudaError_t e = launch_pdl(attn_decode_kernel<C>, dim3((unsigned)(num_sms() * C::CTAS)),
+    cudaError_t e = launch_pdl(attn_decode_kernel<C>, dim3((unsigned)(num_sms() * DEC_CTAS)),
                                dim3(32 * NW), smem, st, p, type);
     return e == cudaSuccess ? JKB_OK : fail_cuda(e, fn);
 }
@@ -696,7 +854,7 @@ int jkb_attn_workspace_create(const jkb_kv_cache *cache, jkb_attn_workspace **ou
     if (!w) return fail(JKB_E_INVALID, fn, 0, 0, 0, "host allocation failed");
     w->device = cache->device;
     w->dim_p = cache->dim_p;
-    w->ctas = 3 * num_sms();
+    w->ctas = DEC_CTAS * num_sms();
     const size_t sms = (size_t)num_sms(), width = (size_t)w->dim_p + 2;
     const size_t part = Arena::round(2 * (size_t)w->ctas * ATTN_ROWS * width * sizeof(float));
     const size_t tile = w->dim_p <= 128 ? Arena::round(2 * sms * 128 * width * sizeof(float)) : 0;

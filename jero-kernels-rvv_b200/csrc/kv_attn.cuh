@@ -2,6 +2,7 @@
 #pragma once
 
 #include "kv_cache.cuh"
+#include "ptx.cuh"
 
 namespace jkb {
 
@@ -47,6 +48,30 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnParams &p, int i) {
     s.lo = 0;
     if (p.window) s.lo = min(max((long long)s.len - s.nq + 1 - p.window, 0ll), (long long)s.len);
     return s;
+}
+
+// A bounded wait in few instructions (the roles' loops hold many): at most 2^20 tries of about a
+// microsecond.
+__device__ __forceinline__ bool mbar_wait_short(uint64_t *b, uint32_t parity,
+                                                volatile int *abort_flag, int *err) {
+#pragma unroll 1
+    for (uint32_t i = 0;; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(b)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (*abort_flag || i >> 20) break;
+    }
+    if (!*abort_flag) {
+        *abort_flag = 1;
+        atomicOr(err, ERR_ATTN_WAIT);
+    }
+    return false;
 }
 
 int attn_decode_launch(const AttnParams &p, int type, int dim_p, size_t max_rows,

@@ -195,30 +195,6 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
         : "memory");
 }
 
-// A bounded wait in few instructions (the roles' loops hold many): at most 2^20 tries of about a
-// microsecond.
-__device__ __forceinline__ bool mbar_wait_short(uint64_t *b, uint32_t parity,
-                                                volatile int *abort_flag, int *err) {
-#pragma unroll 1
-    for (uint32_t i = 0;; i++) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(smem_u32(b)), "r"(parity)
-            : "memory");
-        if (ok) return true;
-        if (*abort_flag || i >> 20) break;
-    }
-    if (!*abort_flag) {
-        *abort_flag = 1;
-        atomicOr(err, ERR_ATTN_WAIT);
-    }
-    return false;
-}
-
 // Two bytes (byte 0 and 1, or 2 and 3, of code + 128) as f16: 0x6400 | byte is 1024 + byte.
 __device__ __forceinline__ uint32_t pair_f16(uint32_t w, uint32_t sel) {
     uint32_t a = __byte_perm(w, 0x64646464u, sel);
