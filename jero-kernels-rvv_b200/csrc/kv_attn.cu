@@ -44,6 +44,9 @@ constexpr int NW = 4;        // warps of a CTA
 constexpr int DEC_CTAS = 2;
 
 constexpr int ND = 3;                  // digits of a query element
+// Pieces of a row tile that are joined at a time, in a tree whose shape only the line decides. (One
+// CTA that joins all 38 pieces of a kv head takes 7.6 us, 4.1 with the tree; of 150, 25 and 6.)
+constexpr int JOIN = 8, JOIN_LEVELS = 3;
 
 template <int DT_, int ROWS_>
 struct DecCfg {
@@ -56,13 +59,14 @@ struct DecCfg {
     static constexpr int UNIT = NW * STEP;        // of a unit
     static constexpr int BATCH = 32 / G;          // steps that are looked up together
     static constexpr int GROUP_BYTES = 32 * DIM;
-    static constexpr int PASSES = 2;
+    static constexpr int PASSES = ROWS * DIM > 1024 ? 4 : 2;
     static constexpr int PASS = DIM / PASSES;  // dims merged at a time
 };
 
+template <int G>
 struct StepInfo {
-    uint32_t src[2];  // the groups' numbers in the cache, + 1; 0: no visible token in it
-    float2 sc[2];     // (ks, vs)
+    float2 sc[G];     // (ks, vs)
+    uint32_t src[G];  // the groups' numbers in the cache, + 1; 0: no visible token in it
     int seq, item;    // item: kv head * row tiles + row tile
     int t0;           // first token (a multiple of 16), and the flags
 };
@@ -72,9 +76,13 @@ enum { STEP_FIRST = 1, STEP_LAST = 2, STEP_WHOLE = 4, STEP_FLAGS = 15 };
 template <class C>
 struct DecSmem {
     alignas(128) uint8_t ring[NW][C::STAGES][C::G * C::GROUP_BYTES];
-    alignas(16) float merge[NW][C::ROWS][C::PASS + 4];
+    union {
+        alignas(16) float merge[NW][C::ROWS][C::PASS + 4];  // while a piece ends
+        alignas(16) uint8_t digits[C::ROWS][ND][C::DIM + 32];  // while one begins (+ 32: banks)
+    };
     float row_m[NW][C::ROWS], row_l[NW][C::ROWS];
-    StepInfo info[NW][2 * C::BATCH];
+    float unit[C::ROWS];
+    StepInfo<C::G> info[NW][2 * C::BATCH];
     uint64_t full[NW][C::STAGES];
     long long warp_sum[NW];
     int abort_flag, is_last;
@@ -133,41 +141,28 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
-// Elements i .. i + 7 of a query row.
-__device__ __forceinline__ void load8(const AttnParams &p, int type, size_t i, float (&x)[8]) {
+// Elements i .. i + 3 of the query rows.
+__device__ __forceinline__ float4 load4(const AttnParams &p, int type, size_t i) {
     if (type == JKB_F32) {
         const float *q = static_cast<const float *>(p.q) + i;
-        if (p.q_vec) {
-            const float4 a = __ldg(reinterpret_cast<const float4 *>(q));
-            const float4 b = __ldg(reinterpret_cast<const float4 *>(q) + 1);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-            x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; k++) x[k] = __ldg(q + k);
-        }
-        return;
+        if (p.q_vec) return __ldg(reinterpret_cast<const float4 *>(q));
+        return make_float4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
     }
     const uint16_t *q = static_cast<const uint16_t *>(p.q) + i;
-    uint32_t w[4];
+    uint2 w;
     if (p.q_vec) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(q));
-        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        w = __ldg(reinterpret_cast<const uint2 *>(q));
     } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            w[k] = __ldg(q + 2 * k) | (uint32_t)__ldg(q + 2 * k + 1) << 16;
+        w.x = __ldg(q) | (uint32_t)__ldg(q + 1) << 16;
+        w.y = __ldg(q + 2) | (uint32_t)__ldg(q + 3) << 16;
     }
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        if (type == JKB_F16) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
-            x[2 * k] = f.x, x[2 * k + 1] = f.y;
-        } else {
-            x[2 * k] = __uint_as_float(w[k] << 16);
-            x[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
-        }
+    if (type == JKB_F16) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+        return make_float4(a.x, a.y, b.x, b.y);
     }
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u),
+                       __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
 }
 
 // Four output elements.
@@ -356,7 +351,7 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
     };
     auto enter = [&](int base, const Look &f, uint32_t src, float2 sc) {
         __syncwarp();
-        StepInfo &i = sm.info[warp][(base + lane / G) % (2 * BATCH)];
+        StepInfo<G> &i = sm.info[warp][(base + lane / G) % (2 * BATCH)];
         i.src[lane % G] = src;
         i.sc[lane % G] = sc;
         if (lane % G == 0) {
@@ -394,10 +389,10 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
         if (phase == 0) look = find(s + BATCH);
         if (phase == BATCH / 2 - 2) look_src = place(look, look_sc);
         if (phase == BATCH - STAGES - 1) enter(s - phase + BATCH, look, look_src, look_sc);
-        StepInfo f = sm.info[warp][s % (2 * BATCH)];
+        StepInfo<G> f = sm.info[warp][s % (2 * BATCH)];
         const int flags = f.t0 & STEP_FLAGS;
         f.t0 &= ~STEP_FLAGS;
-        const bool any = f.src[0] || (G > 1 && f.src[1]);
+        const bool any = f.src[0] || (G > 1 && f.src[G - 1]);
         // (past the last step nothing is looked up, and nothing copied)
         const uint32_t next_src[2] = {sm.info[warp][(s + STAGES) % (2 * BATCH)].src[0],
                                       sm.info[warp][(s + STAGES) % (2 * BATCH)].src[G - 1]};
@@ -406,53 +401,68 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
             const AttnSeq q = attn_seq(p, f.seq);
             const int tiles = (int)(((long long)q.nq * p.group + ROWS - 1) / ROWS);
             const int head = f.item / tiles, tile = f.item - head * tiles;
-#pragma unroll
-            for (int r = 0; r < RH; r++) {
-                const int row = tile * ROWS + g + 8 * r;
-                const int tok = row / p.group;
-                const bool on = tok < q.nq;
+            // each warp brings its share of the rows into digits, for all
+            constexpr int DL = (DIM + 127) / 128;  // 4-element pieces of a lane
+#pragma unroll 2
+            for (int r = warp; r < ROWS; r += NW) {
+                const int row = tile * ROWS + r, tok = row / p.group;
                 const size_t at = (size_t)(q.q0 + tok) * p.q_token +
                                   (size_t)(head * p.group + row - tok * p.group) * p.q_head;
-                float x[DT][8], top = 0.0f;
-                bool finite = true;
+                float4 x[DL];
+                uint32_t top = 0;  // as bits: a NaN is above an infinity is above the rest
 #pragma unroll
-                for (int c = 0; c < DT; c++) {
-                    const int d = 32 * c + 8 * tg;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[c][i] = 0.0f;
-                    if (on && d < p.dim) load8(p, type, at + d, x[c]);
+                for (int k = 0; k < DL; k++) {
+                    const int d = 128 * k + 4 * lane;
+                    x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (tok < q.nq && d < p.dim) x[k] = load4(p, type, at + d);
+                    const uint32_t a = max(__float_as_uint(x[k].x) & 0x7FFFFFFFu,
+                                           __float_as_uint(x[k].y) & 0x7FFFFFFFu);
+                    const uint32_t b = max(__float_as_uint(x[k].z) & 0x7FFFFFFFu,
+                                           __float_as_uint(x[k].w) & 0x7FFFFFFFu);
+                    top = max(top, max(a, b));
                 }
+                top = __reduce_max_sync(~0u, top);
+                const bool finite = top < 0x7F800000u;
+                const float amax = __uint_as_float(top);
+                const float inv = finite && amax > 1e-30f ? __fdividef(MOST, amax) : 0.0f;
 #pragma unroll
-                for (int c = 0; c < DT; c++)
+                for (int k = 0; k < DL; k++) {
+                    const int d = 128 * k + 4 * lane;
+                    if (DIM % 128 && d >= DIM) break;
+                    uint32_t w[4];
+                    w[0] = (uint32_t)(__float2int_rn(x[k].x * inv) + 0x808080) ^ 0x808080u;
+                    w[1] = (uint32_t)(__float2int_rn(x[k].y * inv) + 0x808080) ^ 0x808080u;
+                    w[2] = (uint32_t)(__float2int_rn(x[k].z * inv) + 0x808080) ^ 0x808080u;
+                    w[3] = (uint32_t)(__float2int_rn(x[k].w * inv) + 0x808080) ^ 0x808080u;
+                    const uint32_t a = __byte_perm(w[0], w[1], 0x5140);
+                    const uint32_t b = __byte_perm(w[2], w[3], 0x5140);
+                    *reinterpret_cast<uint32_t *>(&sm.digits[r][2][d]) =
+                        __byte_perm(a, b, 0x5410);
+                    *reinterpret_cast<uint32_t *>(&sm.digits[r][1][d]) =
+                        __byte_perm(a, b, 0x7632);
+                    *reinterpret_cast<uint32_t *>(&sm.digits[r][0][d]) =
+                        __byte_perm(__byte_perm(w[0], w[1], 0x0062),
+                                    __byte_perm(w[2], w[3], 0x0062), 0x5410);
+                }
+                if (lane == 0)
+                    sm.unit[r] =
+                        (finite ? amax / MOST : __int_as_float(0x7FC00000)) * p.scale2;
+            }
+            __syncthreads();
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        finite &= isfinite(x[c][i]);
-                        top = fmaxf(top, fabsf(x[c][i]));
+            for (int r = 0; r < RH; r++) {
+#pragma unroll
+                for (int k = 0; k < ND; k++)
+#pragma unroll
+                    for (int c = 0; c < DT; c++) {
+                        const uint2 w = *reinterpret_cast<const uint2 *>(
+                            &sm.digits[g + 8 * r][k][32 * c + 8 * tg]);
+                        qa[k][c][2 * r] = w.x;
+                        qa[k][c][2 * r + 1] = w.y;
                     }
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                const unsigned all = __ballot_sync(~0u, finite);
-                finite = ((all >> (lane & ~3)) & 15u) == 15u;
-                const float inv = finite && top > 1e-30f ? __fdividef(MOST, top) : 0.0f;
-                unit[r] = (finite ? top / MOST : __int_as_float(0x7FC00000)) * p.scale2;
-#pragma unroll
-                for (int c = 0; c < DT; c++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float y = finite ? x[c][4 * h + i] * inv : 0.0f;
-                            w[i] = (uint32_t)(__float2int_rn(y) + 0x808080) ^ 0x808080u;
-                        }
-                        const uint32_t a = __byte_perm(w[0], w[1], 0x5140);
-                        const uint32_t b = __byte_perm(w[2], w[3], 0x5140);
-                        qa[2][c][2 * r + h] = __byte_perm(a, b, 0x5410);
-                        qa[1][c][2 * r + h] = __byte_perm(a, b, 0x7632);
-                        qa[0][c][2 * r + h] =
-                            __byte_perm(__byte_perm(w[0], w[1], 0x0062),
-                                        __byte_perm(w[2], w[3], 0x0062), 0x5410);
-                    }
+                unit[r] = sm.unit[g + 8 * r];
+                const int tok = (tile * ROWS + g + 8 * r) / p.group;
+                const bool on = tok < q.nq;
                 const int pos = q.len - q.nq + tok;
                 hi[r] = !on ? 0 : p.causal ? min(q.len, pos + 1) : q.len;
                 lo[r] = p.window ? max(0, pos - p.window + 1) : 0;
@@ -520,7 +530,7 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
                             fmaf((float)d0, 65536.0f, fmaf((float)d1, 256.0f, (float)d2)) * f_row;
                     }
                 }
-            if (f.t0 < all_lo || f.t0 + C::STEP > all_hi || (G > 1 && !(f.src[0] && f.src[1]))) {
+            if (f.t0 < all_lo || f.t0 + C::STEP > all_hi || (G > 1 && !(f.src[0] && f.src[G - 1]))) {
 #pragma unroll
                 for (int r = 0; r < RH; r++)
 #pragma unroll
@@ -664,11 +674,17 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
             float top = -INFINITY;
             for (int w = 0; w < NW; w++) top = fmaxf(top, sm.row_m[w][g + 8 * r]);
             mul[r] = ex2(m[r] - (top == -INFINITY ? 0.0f : top));
+            if (tg == 0) sm.row_l[warp][g + 8 * r] *= mul[r];
         }
         // where this piece's sums go: the output, or its slot in the workspace
         const bool whole = flags & STEP_WHOLE;
+        const int rows = min(ROWS, q.nq * p.group - tile * ROWS);
+        int cta0 = 0, cta1 = 0;  // that have a piece of this row tile
         const long long start = prefix[f.seq] + (long long)f.item * units;
-        const int cta0 = (int)(start / per), cta1 = (int)((start + units - 1) / per);
+        if (!whole) {
+            cta0 = (int)(start / per);
+            cta1 = (int)((start + units - 1) / per);
+        }
         auto slot_of = [&](int cta) {
             const int slot = 2 * cta + (cta == cta0 && start != per * cta0 ? 1 : 0);
             return p.partial + (size_t)slot * ROWS * (DIM + 2);
@@ -676,7 +692,7 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
         float *mine = whole ? nullptr : slot_of((int)blockIdx.x);
         auto finish = [&](int row, int d, float4 v, float top, float sum) {
             const int rr = tile * ROWS + row, tok = rr / p.group;
-            if (tok >= q.nq || d >= p.dim) return;
+            if (d >= p.dim) return;
             const int h = head * p.group + rr - tok * p.group;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             store4(p, type, (size_t)(q.q0 + tok) * p.out_token + (size_t)h * p.out_head + d,
@@ -694,7 +710,7 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
                         const int d = 32 * c + 8 * tg + 4 * k - pass * C::PASS;
-                        if (d >= 0 && d < C::PASS) {
+                        if (d >= 0 && d < C::PASS && g + 8 * r < rows) {
                             float x[4];
 #pragma unroll
                             for (int j = 0; j < 4; j++) {
@@ -709,16 +725,15 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
                 }
             }
             __syncthreads();
-            for (int i = tid; i < ROWS * C::PASS / 4; i += 32 * NW) {
+            for (int i = tid; i < rows * C::PASS / 4; i += 32 * NW) {
                 const int row = i / (C::PASS / 4), d = 4 * (i - row * (C::PASS / 4));
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                 float top = -INFINITY, sum = 0.0f;
-                for (int w = 0; w < NW; w++) top = fmaxf(top, sm.row_m[w][row]);
-                const float ref = top == -INFINITY ? 0.0f : top;
                 for (int w = 0; w < NW; w++) {
+                    top = fmaxf(top, sm.row_m[w][row]);
                     const float4 x = *reinterpret_cast<const float4 *>(&sm.merge[w][row][d]);
                     v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-                    sum += sm.row_l[w][row] * ex2(sm.row_m[w][row] - ref);
+                    sum += sm.row_l[w][row];
                 }
                 const int dd = d + pass * C::PASS;
                 if (whole) {
@@ -734,55 +749,74 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
             __syncthreads();
         }
         if (whole) continue;
-        // ---- the last piece of the row tile to arrive adds them all, in order ----
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-            const int before = atomicAdd(&p.counters[cta0], 1);
-            sm.is_last = before == cta1 - cta0;
-            if (sm.is_last) p.counters[cta0] = 0;
-        }
-        __syncthreads();
-        if (!sm.is_last) continue;
-        __threadfence();
-        for (int i = tid; i < ROWS * DIM / 4; i += 32 * NW) {
-            const int row = i / (DIM / 4), d = 4 * (i - row * (DIM / 4));
-            // one pass, the loads of NC pieces in flight together (20 were no faster over 38 pieces and
-            // slower over a few)
-            constexpr int NC = 8;
-            float top = -INFINITY, sum = 0.0f;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        // ---- JOIN pieces into one at a time: the last of them to arrive does, in order ----
+        const int n = cta1 - cta0 + 1;
+        int at = (int)blockIdx.x - cta0;  // this CTA has the sum of pieces at .. at + span - 1
+        for (int span = 1, level = 0; span < n; span *= JOIN, level++) {
+            at -= at % (span * JOIN);
+            const int cnt = min(JOIN, (n - at + span - 1) / span);
+            if (cnt == 1) continue;
+            // (pieces follow in the next CTA too, so no other row tile counts here)
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                int *counter = p.counters + level * gridDim.x + cta0 + at;
+                sm.is_last = atomicAdd(counter, 1) == cnt - 1;
+                if (sm.is_last) *counter = 0;
+            }
+            __syncthreads();
+            if (!sm.is_last) break;
+            __threadfence();
+            const bool all = cnt * span >= n;  // (so at == 0)
+            float *into = slot_of(cta0 + at);
+            for (int i = tid; i < rows * DIM / 4; i += 32 * NW) {
+                const int row = i / (DIM / 4), d = 4 * (i - row * (DIM / 4));
+                constexpr int NC = 8;  // loads in flight together
+                static_assert(JOIN % NC == 0, "");
+                float top = -INFINITY, sum = 0.0f;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-            for (int c0 = cta0; c0 <= cta1; c0 += NC) {
-                float m_in[NC], l_in[NC];
-                float4 v_in[NC];
+                for (int c0 = 0; c0 < cnt; c0 += NC) {
+                    float m_in[NC], l_in[NC];
+                    float4 v_in[NC];
 #pragma unroll
-                for (int k = 0; k < NC; k++) {
-                    const float *slot = slot_of(min(c0 + k, cta1));
-                    m_in[k] = __ldcg(slot + ROWS * DIM + row);
-                    l_in[k] = __ldcg(slot + ROWS * DIM + ROWS + row);
-                    v_in[k] = __ldcg(reinterpret_cast<const float4 *>(slot + row * DIM + d));
+                    for (int k = 0; k < NC; k++) {
+                        const float *slot = slot_of(cta0 + at + min(c0 + k, cnt - 1) * span);
+                        m_in[k] = __ldcg(slot + ROWS * DIM + row);
+                        l_in[k] = __ldcg(slot + ROWS * DIM + ROWS + row);
+                        v_in[k] = __ldcg(reinterpret_cast<const float4 *>(slot + row * DIM + d));
+                    }
+                    float mn = top;
+#pragma unroll
+                    for (int k = 0; k < NC; k++) mn = fmaxf(mn, m_in[k]);
+                    const float ref = mn == -INFINITY ? 0.0f : mn;
+                    const float a = ex2(top - ref);
+                    top = mn;
+                    sum *= a;
+                    v.x *= a, v.y *= a, v.z *= a, v.w *= a;
+#pragma unroll
+                    for (int k = 0; k < NC; k++) {
+                        if (c0 + k >= cnt) continue;
+                        const float w = ex2(m_in[k] - ref);
+                        sum = fmaf(w, l_in[k], sum);
+                        v.x = fmaf(w, v_in[k].x, v.x);
+                        v.y = fmaf(w, v_in[k].y, v.y);
+                        v.z = fmaf(w, v_in[k].z, v.z);
+                        v.w = fmaf(w, v_in[k].w, v.w);
+                    }
                 }
-                float mn = top;
-#pragma unroll
-                for (int k = 0; k < NC; k++) mn = fmaxf(mn, m_in[k]);
-                const float ref = mn == -INFINITY ? 0.0f : mn;
-                const float a = ex2(top - ref);
-                top = mn;
-                sum *= a;
-                v.x *= a, v.y *= a, v.z *= a, v.w *= a;
-#pragma unroll
-                for (int k = 0; k < NC; k++) {
-                    if (c0 + k > cta1) continue;
-                    const float w = ex2(m_in[k] - ref);
-                    sum = fmaf(w, l_in[k], sum);
-                    v.x = fmaf(w, v_in[k].x, v.x);
-                    v.y = fmaf(w, v_in[k].y, v.y);
-                    v.z = fmaf(w, v_in[k].z, v.z);
-                    v.w = fmaf(w, v_in[k].w, v.w);
+                if (all) {
+                    finish(row, d, v, top, sum);
+                } else {
+                    *reinterpret_cast<float4 *>(into + row * DIM + d) = v;
+                    if (d == 0) sm.row_m[0][row] = top, sm.row_l[0][row] = sum;
                 }
             }
-            finish(row, d, v, top, sum);
+            __syncthreads();
+            if (!all && tid < rows) {  // after every thread has read the pieces' own
+                into[ROWS * DIM + tid] = sm.row_m[0][tid];
+                into[ROWS * DIM + ROWS + tid] = sm.row_l[0][tid];
+            }
         }
         __syncthreads();
     }
@@ -797,7 +831,13 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
 }
 
 template <class C>
+constexpr bool dec_fits() {  // DEC_CTAS an SM, for up to 200 sequences (beyond, one may)
+    return DEC_CTAS * (sizeof(DecSmem<C>) + 128 + 8 * 201 + 1024) <= 228 * 1024;
+}
+
+template <class C>
 int launch_cfg(const AttnParams &p, int type, cudaStream_t st) {
+    static_assert(dec_fits<C>(), "");
     static const char *fn = "attention_kv8";
     const size_t smem = sizeof(DecSmem<C>) + 128 + 8 * ((size_t)p.n_seqs + 1);
     static thread_local size_t allowed = 0;
@@ -858,13 +898,17 @@ int jkb_attn_workspace_create(const jkb_kv_cache *cache, jkb_attn_workspace **ou
     const size_t sms = (size_t)num_sms(), width = (size_t)w->dim_p + 2;
     const size_t part = Arena::round(2 * (size_t)w->ctas * ATTN_ROWS * width * sizeof(float));
     const size_t tile = w->dim_p <= 128 ? Arena::round(2 * sms * 128 * width * sizeof(float)) : 0;
-    const size_t counts = (w->ctas + sms) * sizeof(int);
+    const size_t counts = (JOIN_LEVELS * w->ctas + sms) * sizeof(int);
+    if (w->ctas > JOIN * JOIN * JOIN) {
+        free(w);
+        return fail(JKB_E_CAPABILITY, fn, 0, 0, 0, "device has too many SMs");
+    }
     cudaError_t e = cudaMalloc(&w->base, part + tile + counts);
     if (e == cudaSuccess) {
         w->partial = (float *)w->base;
         w->tile_partial = tile ? (float *)(w->base + part) : nullptr;
         w->counters = (int *)(w->base + part + tile);
-        w->tile_counters = w->counters + w->ctas;
+        w->tile_counters = w->counters + JOIN_LEVELS * w->ctas;
         e = cudaMemset(w->counters, 0, counts);
         if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
         if (e != cudaSuccess) cudaFree(w->base);

@@ -36,7 +36,7 @@ struct jkb_attn_workspace {
     uint8_t *base;
     float *partial;       // [2 * ctas][ATTN_ROWS][dim_p + 2]
     float *tile_partial;  // [2 * SMs][dim_p + 2][128]; nullptr above 128 dims
-    int *counters;        // [ctas]
+    int *counters;        // [3][ctas]
     int *tile_counters;   // [SMs]
 };
 
