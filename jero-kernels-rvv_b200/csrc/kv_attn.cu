@@ -44,9 +44,6 @@ constexpr int NW = 4;        // warps of a CTA
 constexpr int DEC_CTAS = 2;
 
 constexpr int ND = 3;                  // digits of a query element
-// Pieces of a row tile that are joined at a time, in a tree whose shape only the line decides. (One
-// CTA that joins all 38 pieces of a kv head takes 7.6 us, 4.1 with the tree; of 150, 25 and 6.)
-constexpr int JOIN = 8, JOIN_LEVELS = 3;
 
 template <int DT_, int ROWS_>
 struct DecCfg {
@@ -898,7 +895,7 @@ int jkb_attn_workspace_create(const jkb_kv_cache *cache, jkb_attn_workspace **ou
     const size_t sms = (size_t)num_sms(), width = (size_t)w->dim_p + 2;
     const size_t part = Arena::round(2 * (size_t)w->ctas * ATTN_ROWS * width * sizeof(float));
     const size_t tile = w->dim_p <= 128 ? Arena::round(2 * sms * 128 * width * sizeof(float)) : 0;
-    const size_t counts = (JOIN_LEVELS * w->ctas + sms) * sizeof(int);
+    const size_t counts = JOIN_LEVELS * (w->ctas + sms) * sizeof(int);
     if (w->ctas > JOIN * JOIN * JOIN) {
         free(w);
         return fail(JKB_E_CAPABILITY, fn, 0, 0, 0, "device has too many SMs");

@@ -657,100 +657,114 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int rr = cur.row0 + row, tok = rr / p.group, h = cur.head * p.group + rr - tok * p.group;
             const size_t at = (size_t)(cur.q0 + tok) * p.out_token + (size_t)h * p.out_head;
             const bool on = tok < cur.nq;
-            if (cur.cta0 == cur.cta1 && p.out_vec) {
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                if (on) {
-                    if (p.lse)
-                        p.lse[(size_t)(cur.q0 + tok) * p.group * p.kv_heads + h] =
-                            (m + log2f(l)) * 0.69314718055994531f;
-                    // column 32 c + 8 j + g of o is dim 32 c + 4 g + j
-#pragma unroll
-                    for (int c = 0; c < DT; c++)
-#pragma unroll
-                        for (int g = 0; g < 8; g += 2) {
-                            float x[8];
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {  // columns 8 i + g and 8 i + g + 1
-                                upk2(o[16 * c + 4 * i + g / 2], x[i], x[4 + i]);
-                                x[i] *= inv;
-                                x[4 + i] *= inv;
-                            }
-                            if (32 * c + 4 * g < p.dim)
-                                store8<C::TYPE>(p, at + 32 * c + 4 * g, x, true);
-                        }
-                }
-                __syncwarp();
-                continue;
-            }
-            // A tile of several CTAs, each with a slot (two where a CTA starts within one such
-            // tile and ends within another), or rows that are not aligned for wide stores: by
-            // way of the workspace
-            {
-                auto slot_of = [&](int cta) {
-                    const int slot = 2 * cta + (cta == cur.cta0 ? 1 : 0);
-                    return p.tile_partial + (size_t)slot * TM * (DIM + 2) + row;
-                };
-                float *mine = slot_of((int)blockIdx.x);
+            // A tile of several CTAs: each leaves its (m, l, o) in a slot of the workspace (two
+            // slots where a CTA starts within one such tile and ends within another)
+            auto slot_of = [&](int cta) {
+                const int slot = 2 * cta + (cta == cur.cta0 ? 1 : 0);
+                return p.tile_partial + (size_t)slot * TM * (DIM + 2) + row;
+            };
+            auto put = [&](float *slot) {
+                if (!on) return;
 #pragma unroll
                 for (int i = 0; i < DIM / 2; i++) {
                     float u, w;
                     upk2(o[i], u, w);
-                    mine[2 * i * TM] = u;
-                    mine[(2 * i + 1) * TM] = w;
+                    slot[2 * i * TM] = u;
+                    slot[(2 * i + 1) * TM] = w;
                 }
-                mine[DIM * TM] = m;
-                mine[(DIM + 1) * TM] = l;
-                bool last = true;
-                if (cur.cta0 != cur.cta1) {
-                    __threadfence();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sm.merge);
-                    if (!wait(&sm.merge, merges++)) goto out;
-                    if (row == 0) {
-                        const int before = atomicAdd(&p.tile_counters[cur.cta0], 1);
-                        sm.is_last = before == cur.cta1 - cur.cta0;
-                        if (sm.is_last) p.tile_counters[cur.cta0] = 0;
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sm.merge);
-                    if (!wait(&sm.merge, merges++)) goto out;
-                    last = *(volatile int *)&sm.is_last;
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sm.merge);  // is_last may be written again
-                    if (!wait(&sm.merge, merges++)) goto out;
-                    __threadfence();
-                }
-                if (!last) continue;
-                m = -INFINITY;
-                for (int k = cur.cta0; k <= cur.cta1; k++) m = fmaxf(m, __ldcg(slot_of(k) + DIM * TM));
-                const float ref = m == -INFINITY ? 0.0f : m;
-                l = 0.0f;
-                for (int k = cur.cta0; k <= cur.cta1; k++)
-                    l = fmaf(ex2(__ldcg(slot_of(k) + DIM * TM) - ref),
-                             __ldcg(slot_of(k) + (DIM + 1) * TM), l);
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                if (on && p.lse)
-                    p.lse[(size_t)(cur.q0 + tok) * p.group * p.kv_heads + h] =
-                        (m + log2f(l)) * 0.69314718055994531f;
-#pragma unroll 1
-                for (int d = 0; d < p.dim; d += 8) {
-                    float x[8] = {};
-#pragma unroll 1
-                    for (int k = cur.cta0; k <= cur.cta1; k++) {
-                        const float *slot = slot_of(k);
-                        const float w = ex2(__ldcg(slot + DIM * TM) - ref);
-                        // dim 32 c + 4 g + j is column 32 c + 8 j + g
-                        const float *col = slot + ((d & ~31) + ((d & 31) >> 2)) * TM;
-#pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            x[i] = fmaf(w, __ldcg(col + (8 * (i & 3) + (i >> 2)) * TM), x[i]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] *= inv;
-                    if (on) store8<C::TYPE>(p, at + d, x, p.out_vec);
+                slot[DIM * TM] = m;
+                slot[(DIM + 1) * TM] = l;
+            };
+            const int n = cur.cta1 - cur.cta0 + 1;
+            int at_cta = (int)blockIdx.x - cur.cta0;  // has the sum of pieces at_cta .. + span - 1
+            bool mine = true;
+            for (int span = 1, level = 0; span < n; span *= JOIN, level++) {
+                const int base = at_cta - at_cta % (span * JOIN);
+                const int cnt = min(JOIN, (n - base + span - 1) / span);
+                if (cnt > 1) put(slot_of(cur.cta0 + at_cta));
+                at_cta = base;
+                if (cnt == 1) continue;
+                __threadfence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.merge);
+                if (!wait(&sm.merge, merges++)) goto out;
+                if (row == 0) {
+                    int *counter = p.tile_counters + level * gridDim.x + cur.cta0 + base;
+                    sm.is_last = atomicAdd(counter, 1) == cnt - 1;
+                    if (sm.is_last) *counter = 0;
                 }
                 __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.merge);
+                if (!wait(&sm.merge, merges++)) goto out;
+                mine = *(volatile int *)&sm.is_last;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.merge);  // is_last may be written again
+                if (!wait(&sm.merge, merges++)) goto out;
+                if (!mine) break;
+                __threadfence();
+                m = -INFINITY;
+                l = 0.0f;
+#pragma unroll
+                for (int i = 0; i < DIM / 2; i++) o[i] = 0;
+                if (!on) continue;
+#pragma unroll 1
+                for (int k = 0; k < cnt; k++)
+                    m = fmaxf(m, __ldcg(slot_of(cur.cta0 + base + k * span) + DIM * TM));
+                const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll 1
+                for (int k = 0; k < cnt; k++) {
+                    const float *slot = slot_of(cur.cta0 + base + k * span);
+                    const float w = ex2(__ldcg(slot + DIM * TM) - ref);
+                    l = fmaf(w, __ldcg(slot + (DIM + 1) * TM), l);
+                    const uint64_t w2 = pkf(w, w);
+#pragma unroll
+                    for (int q = 0; q < DT; q++) {
+                        float x[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i++) x[i] = __ldcg(slot + (32 * q + i) * TM);
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            o[16 * q + i] =
+                                fma2(w2, pkf(x[2 * i], x[2 * i + 1]), o[16 * q + i]);
+                    }
+                }
             }
+            __syncwarp();
+            if (!mine) continue;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            if (on && p.lse)
+                p.lse[(size_t)(cur.q0 + tok) * p.group * p.kv_heads + h] =
+                    (m + log2f(l)) * 0.69314718055994531f;
+            // column 32 c + 8 j + g of o is dim 32 c + 4 g + j
+            if (on && p.out_vec) {
+#pragma unroll
+                for (int c = 0; c < DT; c++)
+#pragma unroll
+                    for (int g = 0; g < 8; g += 2) {
+                        float x[8];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {  // columns 8 i + g and 8 i + g + 1
+                            upk2(o[16 * c + 4 * i + g / 2], x[i], x[4 + i]);
+                            x[i] *= inv;
+                            x[4 + i] *= inv;
+                        }
+                        if (32 * c + 4 * g < p.dim)
+                            store8<C::TYPE>(p, at + 32 * c + 4 * g, x, true);
+                    }
+            } else if (on) {  // rows not aligned for wide stores: by way of the CTA's slot
+                float *slot = slot_of((int)blockIdx.x);
+                put(slot);
+#pragma unroll 1
+                for (int d = 0; d < p.dim; d += 8) {
+                    const float *col = slot + ((d & ~31) + ((d & 31) >> 2)) * TM;
+                    float x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        x[i] = __ldcg(col + (8 * (i & 3) + (i >> 2)) * TM) * inv;
+                    store8<C::TYPE>(p, at + d, x, false);
+                }
+            }
+            __syncwarp();
         }
     } else if (wg == 3) {
         // ------------------------------------------------------------ conversion of keys

@@ -37,7 +37,7 @@ struct jkb_attn_workspace {
     float *partial;       // [2 * ctas][ATTN_ROWS][dim_p + 2]
     float *tile_partial;  // [2 * SMs][dim_p + 2][128]; nullptr above 128 dims
     int *counters;        // [3][ctas]
-    int *tile_counters;   // [SMs]
+    int *tile_counters;   // [3][SMs]
 };
 
 namespace jkb {
