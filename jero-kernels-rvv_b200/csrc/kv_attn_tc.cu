@@ -1122,6 +1122,19 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 __syncwarp();
                 i++;
+                // its query rows, on their way to the L2 while the piece before it runs
+                constexpr int SIZE = C::TYPE == JKB_F32 ? 4 : 2;
+                for (int r = lane; r < TM && !end; r += 32) {
+                    const int tok = (t.row0 + r) / p.group;
+                    if (tok >= s.nq) break;
+                    const char *q = static_cast<const char *>(p.q) +
+                                    ((size_t)(s.q0 + tok) * p.q_token +
+                                     (size_t)(head * p.group + t.row0 + r - tok * p.group) *
+                                         p.q_head) * SIZE;
+                    for (int d = 0; d < p.dim * SIZE; d += 128)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(q + d));
+                }
+                __syncwarp();
             }
             if (end) break;
             start += TILE_COST + t.units;
