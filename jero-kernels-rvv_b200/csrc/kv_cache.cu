@@ -231,11 +231,27 @@ __device__ __forceinline__ void append_run(const Run &r, const AppendSide &src, 
     const float old = r.o ? *scale : 0.0f;
     const int quads = dim >> 2;
     float amax = 0.0f;
-    for (int i = tid; i < r.n * quads; i += TEAM) {
-        const int t = i / quads, q = i - t * quads;
-        const float4 v = elem4<TYPE, VEC>(src.data, row0 + t * src.token_stride + 4 * q);
-        amax = fmaxf(amax, fmaxf(fmaxf(fabsf(finite_or_0(v.x)), fabsf(finite_or_0(v.y))),
-                                 fmaxf(fabsf(finite_or_0(v.z)), fabsf(finite_or_0(v.w)))));
+    int t = tid / quads, q = tid - t * quads;
+    const int step_t = TEAM / quads, step_q = TEAM - step_t * quads;
+    while (t < r.n) {
+        constexpr int U = VEC ? 8 : 2;  // loads in flight
+        float4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (t < r.n) v[u] = elem4<TYPE, VEC>(src.data, row0 + t * src.token_stride + 4 * q);
+            t += step_t;
+            q += step_q;
+            if (q >= quads) {
+                q -= quads;
+                t++;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            amax = fmaxf(amax,
+                         fmaxf(fmaxf(fabsf(finite_or_0(v[u].x)), fabsf(finite_or_0(v[u].y))),
+                               fmaxf(fabsf(finite_or_0(v[u].z)), fabsf(finite_or_0(v[u].w)))));
     }
     for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, d));
     if (TEAM > 32) {
@@ -256,11 +272,64 @@ __device__ __forceinline__ void append_run(const Run &r, const AppendSide &src, 
     const int g0 = grow ? 0 : r.o / KV_GROUP, g1 = (end + KV_GROUP - 1) / KV_GROUP;
     uint8_t *page = codes + bh * (size_t)block_tokens * 2 * dim_p;
     const int patches = dim_p;  // 16 * dim_p bytes of one side of a group
-    for (int i = g0 * patches + tid; i < g1 * patches; i += TEAM) {
+    // the groups that are new as a whole
+    const int f0 = (r.o + KV_GROUP - 1) / KV_GROUP, f1 = max(f0, end / KV_GROUP);
+    const int per = dim_p >> 4;  // key patches of a token
+#pragma unroll 2
+    for (int i = tid; i < (f1 - f0) * patches; i += TEAM) {
+        uint32_t w[4];
+        if (!value) {
+            const int tok = i / per, d0 = 16 * (i - tok * per);
+            const size_t row = row0 + (size_t)(f0 * KV_GROUP + tok - r.o) * src.token_stride;
+            float4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (d0 + 4 * k < dim) v[k] = elem4<TYPE, VEC>(src.data, row + d0 + 4 * k);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                w[k] = pack4(code_of(v[k].x, inv), code_of(v[k].y, inv), code_of(v[k].z, inv),
+                             code_of(v[k].w, inv));
+            uint8_t *g = page + (size_t)(f0 + (tok / KV_GROUP)) * 32 * dim_p;
+            *reinterpret_cast<uint4 *>(g + kv_key_at(tok % KV_GROUP, d0, dim_p)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            const int chunks = i >> 5, q8 = i & 31, tt = q8 >> 3;  // chunks: of 32 dims
+            const int grp = chunks / (dim_p >> 5), chunk = chunks - grp * (dim_p >> 5);
+            const int d0 = 32 * chunk + 4 * ((q8 & 7) ^ (2 * tt));
+            const size_t row =
+                row0 + (size_t)((f0 + grp) * KV_GROUP + 2 * tt - r.o) * src.token_stride + d0;
+            float4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (d0 < dim)
+                    v[k] = elem4<TYPE, VEC>(
+                        src.data, row + (size_t)((k & 1) + 8 * (k >> 1)) * src.token_stride);
+            }
+            const uint32_t b = 0x80808080u;
+            w[0] = b ^ pack4(code_of(v[0].x, inv), code_of(v[1].x, inv), code_of(v[2].x, inv),
+                             code_of(v[3].x, inv));
+            w[1] = b ^ pack4(code_of(v[0].y, inv), code_of(v[1].y, inv), code_of(v[2].y, inv),
+                             code_of(v[3].y, inv));
+            w[2] = b ^ pack4(code_of(v[0].z, inv), code_of(v[1].z, inv), code_of(v[2].z, inv),
+                             code_of(v[3].z, inv));
+            w[3] = b ^ pack4(code_of(v[0].w, inv), code_of(v[1].w, inv), code_of(v[2].w, inv),
+                             code_of(v[3].w, inv));
+            *reinterpret_cast<uint4 *>(page + (size_t)(f0 + grp) * 32 * dim_p + 16 * dim_p +
+                                       512 * chunk + 16 * q8) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    // the groups before and after, which keep bytes or end within
+    const int before = max(f0 - g0, 0) * patches, after = (g1 - f1) * patches;
+    for (int j = tid; j < before + after; j += TEAM) {
+        const int i = j < before ? j + g0 * patches : j - before + f1 * patches;
         const int grp = i / patches, p = i - grp * patches;
         uint8_t *g = page + (size_t)grp * 32 * dim_p;
         if (!value) {
-            const int per = dim_p >> 4, tok = p / per, d0 = 16 * (p - tok * per);
+            const int tok = p / per, d0 = 16 * (p - tok * per);
             const int off = grp * KV_GROUP + tok;
             uint4 *at = reinterpret_cast<uint4 *>(g + kv_key_at(tok, d0, dim_p));
             uint32_t w[4];
@@ -318,9 +387,9 @@ __device__ __forceinline__ void append_run(const Run &r, const AppendSide &src, 
                     c[3][k] = code_of(v.w, inv) + 128;
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        c[j][k] = is_old[k] ? recode<true>(x[j], k, ratio)
-                                            : (int)((x[j] >> (8 * k)) & 255);
+                    for (int e = 0; e < 4; e++)
+                        c[e][k] = is_old[k] ? recode<true>(x[e], k, ratio)
+                                            : (int)((x[e] >> (8 * k)) & 255);
                 }
             }
             *at = make_uint4(pack4(c[0][0], c[0][1], c[0][2], c[0][3]),
@@ -410,12 +479,13 @@ enum { COPY_IMPORT, COPY_EXPORT, COPY_READ };
 
 // One thread a 16-byte patch of codes (a key patch: 16 dims of a token; a value patch: 4 dims of
 // 4 tokens). MODE COPY_READ writes 64 bytes of f32 values for it, which bounds the kernel.
-template <int MODE>
+template <int MODE, int DP>
 __global__ void __launch_bounds__(COPY_THREADS)
     copy_kernel(const int32_t *__restrict__ blocks, uint8_t *__restrict__ codes,
                 float2 *__restrict__ scales, int n_blocks, int n_heads, int block_tokens, int dim,
-                int dim_p, void *__restrict__ k_any, void *__restrict__ v_any,
+                void *__restrict__ k_any, void *__restrict__ v_any,
                 float *__restrict__ k_scales, float *__restrict__ v_scales, int *err) {
+    constexpr int dim_p = DP;
     const int head = blockIdx.y;
     const size_t i = blockIdx.x;
     pdl_enter();
@@ -436,6 +506,7 @@ __global__ void __launch_bounds__(COPY_THREADS)
         v_scales[out_bh] = s.y;
     }
     const int total = block_tokens / KV_GROUP * 2 * dim_p;
+#pragma unroll 2
     for (int p = threadIdx.x; p < total; p += COPY_THREADS) {
         const int grp = p / (2 * dim_p);
         int q = p - grp * 2 * dim_p;
@@ -529,10 +600,16 @@ int copy_launch(const jkb_kv_cache *c, const int32_t *blocks, size_t n, void *k,
     if (n == 0) return JKB_OK;
     int *err = device_error_word();
     if (!err) return fail(JKB_E_CUDA, fn, 0, 0, 0, "no device error word");
-    cudaError_t e = launch_pdl(copy_kernel<MODE>, dim3((unsigned)n, (unsigned)c->n_heads),
-                               dim3(COPY_THREADS), 0, as_stream(stream), blocks, c->codes,
-                               c->scales, (int)c->n_blocks, (int)c->n_heads, c->block_tokens,
-                               c->dim, c->dim_p, k, v, ks, vs, err);
+    auto go = [&](auto kern) {
+        return launch_pdl(kern, dim3((unsigned)n, (unsigned)c->n_heads), dim3(COPY_THREADS), 0,
+                          as_stream(stream), blocks, c->codes, c->scales, (int)c->n_blocks,
+                          (int)c->n_heads, c->block_tokens, c->dim, k, v, ks, vs, err);
+    };
+    cudaError_t e = c->dim_p == 64    ? go(copy_kernel<MODE, 64>)
+                    : c->dim_p == 96  ? go(copy_kernel<MODE, 96>)
+                    : c->dim_p == 128 ? go(copy_kernel<MODE, 128>)
+                    : c->dim_p == 192 ? go(copy_kernel<MODE, 192>)
+                                      : go(copy_kernel<MODE, 256>);
     return e == cudaSuccess ? JKB_OK : fail_cuda(e, fn);
 }
 
