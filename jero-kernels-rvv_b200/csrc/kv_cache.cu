@@ -195,10 +195,14 @@ __device__ __forceinline__ float4 elem4(const void *p, size_t i) {
 
 __device__ __forceinline__ float finite_or_0(float v) { return isfinite(v) ? v : 0.0f; }
 
-// Code of one element: rint(x * inv), ties to even, in [-127, 127].
-__device__ __forceinline__ int code_of(float x, float inv) {
-    const float r = rintf(__fmul_rn(finite_or_0(x), inv));
-    return (int)fminf(fmaxf(r, -127.0f), 127.0f);
+// Code of one element in the low byte: rint(x * inv), ties to even; |x * inv| < 127.5, and adding
+// 1.5 * 2^23 rounds to an integer, whose two's complement the low bits are.
+__device__ __forceinline__ uint32_t code_of(float x, float inv) {
+    return __float_as_uint(__fadd_rn(__fmul_rn(finite_or_0(x), inv), 12582912.0f));
+}
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
     return (a & 255) | (b & 255) << 8 | (c & 255) << 16 | (uint32_t)(d & 255) << 24;
@@ -216,48 +220,61 @@ struct Run {
     int t0, n, o, block;
 };
 
-// Scale and codes of one run, head and side by a team of TEAM threads (a warp or the CTA).
-// A first pass takes the rows' absmax; the second reads them again (from L1: a block's rows are
-// at most 64 KB) and writes 16 bytes of codes at a time: a key patch is 16 dims of one token, a
-// value patch 4 dims of 4 tokens. Old bytes are read only where a patch keeps some of them.
-template <int TYPE, bool VEC, int TEAM>
+// Scale and codes of one run, head and side by a team of threads (a warp or the CTA).
+// A first pass takes the rows' absmax; the second reads them again (from L1 or L2: a block's rows
+// are at most 64 KB) and writes 16 bytes of codes at a time: a key patch is 16 dims of one token,
+// a value patch 4 dims of 4 tokens. Old bytes are read only where a patch keeps some of them.
+// Instructions bound it, their number an element and, as each runs a few times a run, their
+// fetching: the rare paths are loops over little code. (Patches kept in registers between the
+// passes, in eight times the code, took twice as long.)
+template <int TYPE, bool VEC>
 __device__ __forceinline__ void append_run(const Run &r, const AppendSide &src, bool value,
-                                           int head, int tid, uint8_t *codes, float2 *scales,
-                                           int n_heads, int block_tokens, int dim, int dim_p,
-                                           float *red) {
+                                           int head, int tid, int team, uint8_t *codes,
+                                           float2 *scales, int n_heads, int block_tokens, int dim,
+                                           int dim_p, float *red) {
     const size_t row0 = (size_t)r.t0 * src.token_stride + (size_t)head * src.head_stride;
     const size_t bh = (size_t)r.block * n_heads + head;
     float *scale = &scales[bh].x + (value ? 1 : 0);
     const float old = r.o ? *scale : 0.0f;
     const int quads = dim >> 2;
     float amax = 0.0f;
-    int t = tid / quads, q = tid - t * quads;
-    const int step_t = TEAM / quads, step_q = TEAM - step_t * quads;
-    while (t < r.n) {
-        constexpr int U = VEC ? 8 : 2;  // loads in flight
-        float4 v[U];
+    {
+        int t = tid / quads, q = tid - t * quads;
+        const int step_t = team / quads, step_q = team - step_t * quads;
+#pragma unroll 1
+        while (t < r.n) {
+            constexpr int U = VEC ? 8 : 2;  // loads in flight
+            float4 v[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (t < r.n) v[u] = elem4<TYPE, VEC>(src.data, row0 + t * src.token_stride + 4 * q);
-            t += step_t;
-            q += step_q;
-            if (q >= quads) {
-                q -= quads;
-                t++;
+            for (int u = 0; u < U; u++) {
+                v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (t < r.n)
+                    v[u] = elem4<TYPE, VEC>(src.data, row0 + t * src.token_stride + 4 * q);
+                t += step_t;
+                q += step_q;
+                if (q >= quads) {
+                    q -= quads;
+                    t++;
+                }
             }
-        }
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            amax = fmaxf(amax,
-                         fmaxf(fmaxf(fabsf(finite_or_0(v[u].x)), fabsf(finite_or_0(v[u].y))),
-                               fmaxf(fabsf(finite_or_0(v[u].z)), fabsf(finite_or_0(v[u].w)))));
+            for (int u = 0; u < U; u++)  // (fmaxf passes over a NaN)
+                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v[u].x), fabsf(v[u].y)),
+                                         fmaxf(fabsf(v[u].z), fabsf(v[u].w))));
+        }
+        if (amax == INFINITY) {  // infinities count as 0: once more without them
+            amax = 0.0f;
+#pragma unroll 1
+            for (int i = tid; i < r.n * dim; i += team)
+                amax = fmaxf(amax, fabsf(finite_or_0(elem<TYPE>(
+                                       src.data, row0 + i / dim * src.token_stride + i % dim))));
+        }
     }
     for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, d));
-    if (TEAM > 32) {
+    if (team > 32) {
         if ((tid & 31) == 0) red[tid >> 5] = amax;
         __syncthreads();
-        for (int w = 0; w < TEAM / 32; w++) amax = fmaxf(amax, red[w]);
+        for (int w = 0; w < APPEND_THREADS / 32; w++) amax = fmaxf(amax, red[w]);
         __syncthreads();
     } else {
         __syncwarp();
@@ -275,127 +292,103 @@ __device__ __forceinline__ void append_run(const Run &r, const AppendSide &src, 
     // the groups that are new as a whole
     const int f0 = (r.o + KV_GROUP - 1) / KV_GROUP, f1 = max(f0, end / KV_GROUP);
     const int per = dim_p >> 4;  // key patches of a token
-#pragma unroll 2
-    for (int i = tid; i < (f1 - f0) * patches; i += TEAM) {
-        uint32_t w[4];
+#pragma unroll 1
+    for (int i = tid; i < (f1 - f0) * patches; i += team) {
+        // v[k]: dims d0 + 4 k .. of token tok, or dims d0 .. of token tok + (k & 1) + 8 (k >> 1)
+        int tok, d0;
+        uint8_t *at;
+        size_t step[2];
         if (!value) {
-            const int tok = i / per, d0 = 16 * (i - tok * per);
-            const size_t row = row0 + (size_t)(f0 * KV_GROUP + tok - r.o) * src.token_stride;
-            float4 v[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (d0 + 4 * k < dim) v[k] = elem4<TYPE, VEC>(src.data, row + d0 + 4 * k);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                w[k] = pack4(code_of(v[k].x, inv), code_of(v[k].y, inv), code_of(v[k].z, inv),
-                             code_of(v[k].w, inv));
-            uint8_t *g = page + (size_t)(f0 + (tok / KV_GROUP)) * 32 * dim_p;
-            *reinterpret_cast<uint4 *>(g + kv_key_at(tok % KV_GROUP, d0, dim_p)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
+            tok = i / per;
+            d0 = 16 * (i - tok * per);
+            at = page + (size_t)(f0 + (tok / KV_GROUP)) * 32 * dim_p +
+                 kv_key_at(tok % KV_GROUP, d0, dim_p);
+            step[0] = 4, step[1] = 8;
         } else {
             const int chunks = i >> 5, q8 = i & 31, tt = q8 >> 3;  // chunks: of 32 dims
             const int grp = chunks / (dim_p >> 5), chunk = chunks - grp * (dim_p >> 5);
-            const int d0 = 32 * chunk + 4 * ((q8 & 7) ^ (2 * tt));
-            const size_t row =
-                row0 + (size_t)((f0 + grp) * KV_GROUP + 2 * tt - r.o) * src.token_stride + d0;
-            float4 v[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (d0 < dim)
-                    v[k] = elem4<TYPE, VEC>(
-                        src.data, row + (size_t)((k & 1) + 8 * (k >> 1)) * src.token_stride);
-            }
-            const uint32_t b = 0x80808080u;
-            w[0] = b ^ pack4(code_of(v[0].x, inv), code_of(v[1].x, inv), code_of(v[2].x, inv),
-                             code_of(v[3].x, inv));
-            w[1] = b ^ pack4(code_of(v[0].y, inv), code_of(v[1].y, inv), code_of(v[2].y, inv),
-                             code_of(v[3].y, inv));
-            w[2] = b ^ pack4(code_of(v[0].z, inv), code_of(v[1].z, inv), code_of(v[2].z, inv),
-                             code_of(v[3].z, inv));
-            w[3] = b ^ pack4(code_of(v[0].w, inv), code_of(v[1].w, inv), code_of(v[2].w, inv),
-                             code_of(v[3].w, inv));
-            *reinterpret_cast<uint4 *>(page + (size_t)(f0 + grp) * 32 * dim_p + 16 * dim_p +
-                                       512 * chunk + 16 * q8) =
-                make_uint4(w[0], w[1], w[2], w[3]);
+            tok = grp * KV_GROUP + 2 * tt;
+            d0 = 32 * chunk + 4 * ((q8 & 7) ^ (2 * tt));
+            at = page + (size_t)(f0 + grp) * 32 * dim_p + 16 * dim_p + 512 * chunk + 16 * q8;
+            step[0] = src.token_stride, step[1] = 8 * src.token_stride;
         }
+        const size_t row = row0 + (size_t)(f0 * KV_GROUP + tok - r.o) * src.token_stride + d0;
+        uint32_t c[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if ((value ? d0 : d0 + 4 * k) < dim)
+                v = elem4<TYPE, VEC>(src.data,
+                                     row + (k & 1 ? step[0] : 0) + (k >> 1 ? step[1] : 0));
+            c[k][0] = code_of(v.x, inv), c[k][1] = code_of(v.y, inv);
+            c[k][2] = code_of(v.z, inv), c[k][3] = code_of(v.w, inv);
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            w[k] = value ? 0x80808080u ^ low4(c[0][k], c[1][k], c[2][k], c[3][k])
+                         : low4(c[k][0], c[k][1], c[k][2], c[k][3]);
+        *reinterpret_cast<uint4 *>(at) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     // the groups before and after, which keep bytes or end within
     const int before = max(f0 - g0, 0) * patches, after = (g1 - f1) * patches;
-    for (int j = tid; j < before + after; j += TEAM) {
+#pragma unroll 1
+    for (int j = tid; j < before + after; j += team) {
         const int i = j < before ? j + g0 * patches : j - before + f1 * patches;
         const int grp = i / patches, p = i - grp * patches;
         uint8_t *g = page + (size_t)grp * 32 * dim_p;
         if (!value) {
             const int tok = p / per, d0 = 16 * (p - tok * per);
             const int off = grp * KV_GROUP + tok;
-            uint4 *at = reinterpret_cast<uint4 *>(g + kv_key_at(tok, d0, dim_p));
-            uint32_t w[4];
-            if (off >= r.o && off < end) {
-                const size_t row = row0 + (size_t)(off - r.o) * src.token_stride;
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int d = d0 + 4 * k;
-                    w[k] = 0;
-                    if (d < dim) {
-                        const float4 v = elem4<TYPE, VEC>(src.data, row + d);
-                        w[k] = pack4(code_of(v.x, inv), code_of(v.y, inv), code_of(v.z, inv),
-                                     code_of(v.w, inv));
-                    }
+            if (off >= end || (off < r.o && !grow)) continue;
+            uint32_t *at = reinterpret_cast<uint32_t *>(g + kv_key_at(tok, d0, dim_p));
+            const size_t row = row0 + (size_t)(off - r.o) * src.token_stride + d0;
+#pragma unroll 1
+            for (int k = 0; k < 4; k++) {
+                uint32_t w = 0;
+                if (off < r.o) {
+                    const uint32_t x = at[k];
+                    w = pack4(recode<false>(x, 0, ratio), recode<false>(x, 1, ratio),
+                              recode<false>(x, 2, ratio), recode<false>(x, 3, ratio));
+                } else if (d0 + 4 * k < dim) {
+                    const float4 v = elem4<TYPE, VEC>(src.data, row + 4 * k);
+                    w = low4(code_of(v.x, inv), code_of(v.y, inv), code_of(v.z, inv),
+                             code_of(v.w, inv));
                 }
-            } else if (grow && off < r.o) {
-                const uint4 was = *at;
-                const uint32_t x[4] = {was.x, was.y, was.z, was.w};
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    w[k] = pack4(recode<false>(x[k], 0, ratio), recode<false>(x[k], 1, ratio),
-                                 recode<false>(x[k], 2, ratio), recode<false>(x[k], 3, ratio));
-            } else {
-                continue;
+                at[k] = w;
             }
-            *at = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
             const int chunk = p >> 5, q = p & 31, t = q >> 3;
             const int d0 = 32 * chunk + 4 * ((q & 7) ^ (2 * t));
             uint4 *at = reinterpret_cast<uint4 *>(g + 16 * dim_p + 512 * chunk + 16 * q);
-            bool is_new[4], is_old[4], any = false, keep = false;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
+            uint4 was = make_uint4(0, 0, 0, 0);
+            bool any = false;
+#pragma unroll 1
+            for (int k = 0; k < 4; k++) {  // byte k of the words: token 2 t + (k & 1) + 8 (k >> 1)
                 const int off = grp * KV_GROUP + 2 * t + (k & 1) + 8 * (k >> 1);
-                is_new[k] = off >= r.o && off < end;
-                is_old[k] = grow && off < r.o;
-                any |= is_new[k] || is_old[k];
-                keep |= !is_new[k];
-            }
-            if (!any) continue;
-            const uint4 was = keep ? *at : make_uint4(0, 0, 0, 0);
-            const uint32_t x[4] = {was.x, was.y, was.z, was.w};
-            int c[4][4];  // [dim][token]
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if (is_new[k]) {
-                    const int off = grp * KV_GROUP + 2 * t + (k & 1) + 8 * (k >> 1);
+                const bool is_new = off >= r.o && off < end, is_old = grow && off < r.o;
+                if (!is_new && !is_old) continue;
+                if (!any) was = *at;
+                any = true;
+                uint32_t c[4];
+                if (is_new) {
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (d0 < dim)
                         v = elem4<TYPE, VEC>(src.data,
                                              row0 + (size_t)(off - r.o) * src.token_stride + d0);
-                    c[0][k] = code_of(v.x, inv) + 128;
-                    c[1][k] = code_of(v.y, inv) + 128;
-                    c[2][k] = code_of(v.z, inv) + 128;
-                    c[3][k] = code_of(v.w, inv) + 128;
+                    c[0] = code_of(v.x, inv) + 128, c[1] = code_of(v.y, inv) + 128;
+                    c[2] = code_of(v.z, inv) + 128, c[3] = code_of(v.w, inv) + 128;
                 } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        c[e][k] = is_old[k] ? recode<true>(x[e], k, ratio)
-                                            : (int)((x[e] >> (8 * k)) & 255);
+                    c[0] = recode<true>(was.x, k, ratio), c[1] = recode<true>(was.y, k, ratio);
+                    c[2] = recode<true>(was.z, k, ratio), c[3] = recode<true>(was.w, k, ratio);
                 }
+                const uint32_t mask = 255u << (8 * k);
+                was.x = (was.x & ~mask) | (c[0] & 255) << (8 * k);
+                was.y = (was.y & ~mask) | (c[1] & 255) << (8 * k);
+                was.z = (was.z & ~mask) | (c[2] & 255) << (8 * k);
+                was.w = (was.w & ~mask) | (c[3] & 255) << (8 * k);
             }
-            *at = make_uint4(pack4(c[0][0], c[0][1], c[0][2], c[0][3]),
-                             pack4(c[1][0], c[1][1], c[1][2], c[1][3]),
-                             pack4(c[2][0], c[2][1], c[2][2], c[2][3]),
-                             pack4(c[3][0], c[3][1], c[3][2], c[3][3]));
+            if (any) *at = was;
         }
     }
 }
@@ -453,12 +446,9 @@ __global__ void __launch_bounds__(APPEND_THREADS)
             }
         for (int d = 16; d; d >>= 1) n = min(n, __shfl_xor_sync(~0u, n, d));
         const Run r{first + at, n, s & ((1 << log_block) - 1), s >> log_block};
-        if (each)
-            append_run<TYPE, VEC, 32>(r, src, value, head, lane, codes, scales, n_heads,
-                                      1 << log_block, dim, dim_p, red);
-        else
-            append_run<TYPE, VEC, APPEND_THREADS>(r, src, value, head, tid, codes, scales,
-                                                  n_heads, 1 << log_block, dim, dim_p, red);
+        append_run<TYPE, VEC>(r, src, value, head, each ? lane : tid,
+                              each ? 32 : APPEND_THREADS, codes, scales, n_heads, 1 << log_block,
+                              dim, dim_p, red);
     }
 }
 
