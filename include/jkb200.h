@@ -724,7 +724,9 @@ int jkb_kv_cache_destroy(jkb_kv_cache *cache);
 int jkb_kv_cache_info(const jkb_kv_cache *cache, size_t *n_blocks, size_t *block_tokens,
                       size_t *n_kv_heads, size_t *head_dim, size_t *device_bytes);
 /* Copies blocks in and out: `blocks` are n distinct block ids (device); codes are
- * [n][n_kv_heads][block_tokens][head_dim] int8, scales [n][n_kv_heads] f32 (device). */
+ * [n][n_kv_heads][block_tokens][head_dim] int8, scales [n][n_kv_heads] f32 (device). Imported
+ * codes lie in -127 .. 127 and scales are finite and not negative, as jkb_kv_append writes them;
+ * the attention of a cache with others is undefined (but stays within its memory). */
 int jkb_kv_cache_import(jkb_kv_cache *cache, const int32_t *blocks, size_t n,
                         const int8_t *k_codes, const int8_t *v_codes, const float *k_scales,
                         const float *v_scales, void *stream);
@@ -795,7 +797,10 @@ int jkb_attn_workspace_destroy(jkb_attn_workspace *ws);
  * that sees no token has out = 0 and lse = -inf; one with a non-finite element has NaN.
  * q and out share a type; out rows may be strided too. Sums, softmax statistics and the
  * accumulated output are f32 for every type. max_new: an upper bound of the query tokens of a
- * sequence (it selects the kernels; outputs stay right above it, but slow). */
+ * sequence (it selects the kernels; outputs stay right above it, but slow). Sequences of up to 16
+ * query rows (tokens times n_heads / n_kv_heads), and all of head_dim > 128, take the few-row
+ * kernel, where a token whose weight is below 2^-39 of its row's largest counts as 0; the others
+ * take the prompt kernel. Results do not depend on timing: a call repeated gives the same bits. */
 typedef struct {
     const jkb_kv_cache *cache;
     jkb_attn_workspace *ws;

@@ -1395,7 +1395,7 @@ class KvCache:
 
     def import_blocks(self, blocks, k_codes, v_codes, k_scales, v_scales, stream=None):
         """Sets the blocks (distinct int32 ids): codes int8 [n, kv heads, block tokens, head dim],
-        scales float32 [n, kv heads]."""
+        scales float32 [n, kv heads], finite and not negative."""
         a = self._planes(blocks, k_codes, v_codes, torch.int8)
         _check(_L().jkb_kv_cache_import(self.handle, *a, *self._scales(blocks, k_scales, v_scales),
                                         _stream(stream)))
@@ -1428,7 +1428,7 @@ def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Ten
     """Quantizes the key and value rows [tokens, kv heads, head dim] (float32, float16 or
     bfloat16; parts of a fused projection may be strided) into their slots (int32; negative:
     skipped). The tokens of a block stand together, in consecutive slots. A block's scale is its
-    absmax / 127: fresh where its first new token has offset 0, else the larger of its own and the
+    absmax * float32(1 / 127): fresh where its first new token has offset 0, else the larger of its own and the
     new rows', its earlier codes being rounded again where it grew."""
     kr = _rows(k, "k", cache.n_kv_heads, cache.head_dim)
     vr = _rows(v, "v", cache.n_kv_heads, cache.head_dim)
