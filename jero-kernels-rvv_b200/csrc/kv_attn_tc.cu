@@ -45,11 +45,13 @@
 // 1111 cached ones takes 222 us (324 TFLOP/s of its two products; the 5 f16 products that f32
 // needs run at 810), one of 8192 bf16 tokens 1084 us (507 TFLOP/s; with p's second part 761);
 // nine ragged f16 chunks, 5331 tokens of 14 query heads over 2 of 80 dims, 176 us. What bounds a
-// unit are the issue slots above; a tile's start and end cost as much as 7 units.
+// unit are the issue slots above; a tile's start and end cost as much as 5 units.
 #include "kv_attn.cuh"
 #include "ptx.cuh"
 
 #include <cuda_bf16.h>
+
+#include <cfloat>
 
 namespace jkb {
 
@@ -59,7 +61,7 @@ constexpr int TM = 128;        // query rows of a tile
 constexpr int TN = 128;        // cached tokens of a unit
 constexpr int GROUPS = TN / KV_GROUP;
 constexpr int THREADS = 768;
-constexpr int TILE_COST = 7;   // of a tile's start and end, in units (measured: 7 best of 2, 4, 7, 10)
+constexpr int TILE_COST = 5;   // of a tile's start and end, in units (measured: 5 best of 3, 5, 7)
 constexpr int RAW = 2;         // raw rings of codes, units
 constexpr int SC = 8;          // ring of block scales, units
 constexpr int REGS_SOFT = 88, REGS_SUM = 184, REGS_CONV = 40, REGS_REST = 40;  // of a warpgroup
@@ -348,18 +350,45 @@ __device__ __forceinline__ float scale_f16(float vs, int vexp) {
                              : 0.0f;
 }
 
-// One unit of one row (thread): S from TMEM at ts, scaled by rs ks and masked to tokens lo .. hi
-// of the unit; returns (m, l). p's parts go back to TMEM over S: of the 16 columns of a group of
-// tokens, the first 8 take part 0, the last 8 part 1; part 2 stands behind S.
-// S is read twice (maximum, then weights), 32 columns at a time: loops stay rolled where they can: with more unrolling the roles'
-// code outgrows the SM's instruction cache, and every unit fetches it anew (unrolled over 128
-// columns, four times slower).
-// rs and ks are not negative (a negative softmax scale's sign is in Q).
-template <class C, bool MASKED>
+// Tokens outside lo .. hi of the unit, and of groups that are not there, get S = -inf, before
+// softmax_unit, which so needs no test for them: beside a second form of it with the tests, which
+// a tile's last units ran from a cold instruction cache, this took 5 to 9 us less a tile.
+__device__ __forceinline__ void mask_unit(uint32_t ts, uint32_t valid, int lo, int hi) {
+#pragma unroll 1
+    for (int h = 0; h < 4; h++) {
+        const int a = min(max(lo - 32 * h, 0), 32), b = min(max(hi - 32 * h, 0), 32);
+        uint32_t m = (uint32_t)((1ull << b) - 1) & ~(uint32_t)((1ull << a) - 1);
+        if (!((valid >> (2 * h)) & 1)) m &= 0xFFFF0000u;
+        if (!((valid >> (2 * h + 1)) & 1)) m &= 0x0000FFFFu;
+        if (__all_sync(~0u, m == ~0u)) continue;
+        uint32_t r[32];
+        tmem_ld32(ts + 32 * h, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            uint32_t x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                x[i] = m & (1u << (8 * j + i)) ? r[8 * j + i] : 0xFF800000u;
+            tmem_st8(ts + 32 * h + 8 * j, x);
+        }
+    }
+    tmem_st_wait();
+}
+
+// One unit of one row (thread): S from TMEM at ts, scaled by rs ks; returns (m, l). p's parts go
+// back to TMEM over S: of the 16 columns of a group of tokens, the first 8 take part 0, the last
+// 8 part 1; part 2 stands behind S.
+// S is read twice (maximum, then weights), 32 columns at a time: loops stay rolled where they
+// can: with more unrolling the roles' code outgrows the SM's instruction cache, and every unit
+// fetches it anew (unrolled over 128 columns, four times slower).
+// rs and ks are not negative (a negative softmax scale's sign is in Q); where they give 0, the
+// smallest normal number in its place keeps a masked token's -inf.
+template <class C>
 __device__ __forceinline__ float2 softmax_unit(uint32_t ts, const float2 *sc, uint32_t valid,
-                                               float rs, int lo, int hi) {
+                                               float rs) {
     constexpr int NP = C::NP;
-    float top = -INFINITY;
+    float top = -INFINITY, most = -INFINITY;  // of s; of S
     uint32_t r[32];
     tmem_ld32(ts, r);
 #pragma unroll 1
@@ -370,22 +399,18 @@ __device__ __forceinline__ float2 softmax_unit(uint32_t ts, const float2 *sc, ui
             float t2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                float u = __uint_as_float(r[16 * k + 2 * i]);
-                float w = __uint_as_float(r[16 * k + 2 * i + 1]);
-                if (MASKED) {
-                    const int t = 32 * h + 16 * k + 2 * i;
-                    const bool on = (valid >> (2 * h + k)) & 1;
-                    u = on && t >= lo && t < hi ? u : -INFINITY;
-                    w = on && t + 1 >= lo && t + 1 < hi ? w : -INFINITY;
-                }
+                const float u = __uint_as_float(r[16 * k + 2 * i]);
+                const float w = __uint_as_float(r[16 * k + 2 * i + 1]);
                 t2[i & 1] = fmaxf(t2[i & 1], fmaxf(u, w));
             }
             const float raw = fmaxf(t2[0], t2[1]);
+            most = fmaxf(most, raw);
             top = fmaxf(top, raw == -INFINITY ? raw : raw * (rs * sc[2 * h + k].x));
         }
         tmem_ld32(ts + 32 * ((h + 1) & 3), r);
     }
     const float ref = top == -INFINITY ? 0.0f : top;
+    if (most == -INFINITY) rs = 0.0f;  // sees nothing here: no NaN from its scale either
     int vexp = 0;
     if (C::F16) vexp = unit_vexp(sc, valid);
     const uint64_t nref = pkf(-ref, -ref), minus = pkf(-1.0f, -1.0f);
@@ -396,18 +421,14 @@ __device__ __forceinline__ float2 softmax_unit(uint32_t ts, const float2 *sc, ui
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             const int g = 2 * h + k;
-            const float f = rs * sc[g].x, vs = C::F16 ? scale_f16(sc[g].y, vexp) : sc[g].y;
+            float f = rs * sc[g].x;
+            f = f < FLT_MIN ? FLT_MIN : f;
+            const float vs = C::F16 ? scale_f16(sc[g].y, vexp) : sc[g].y;
             uint32_t part[NP][8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 float u, w;
                 upk2(fma2(pk2(r[16 * k + 2 * i], r[16 * k + 2 * i + 1]), pkf(f, f), nref), u, w);
-                if (MASKED) {
-                    const int t = 16 * g + 2 * i;
-                    const bool on = (valid >> g) & 1;
-                    u = on && t >= lo && t < hi ? u : -INFINITY;
-                    w = on && t + 1 >= lo && t + 1 < hi ? w : -INFINITY;
-                }
                 uint64_t e = pkf(ex2(u), ex2(w));
                 sum = add2(sum, e);
                 e = mul2(e, pkf(vs, vs));
@@ -610,11 +631,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const uint32_t valid = sm.valid[i % SC];
                 const float2 *sc = sm.sc[i % SC];
                 const uint32_t ts = tl + b * C::S_COLS;
-                float2 st;
                 if (key0 < cur.all_lo || key0 + TN > cur.all_hi || valid != 0xFFu)
-                    st = softmax_unit<C, true>(ts, sc, valid, rs, lo - key0, hi - key0);
-                else
-                    st = softmax_unit<C, false>(ts, sc, valid, rs, 0, TN);
+                    mask_unit(ts, valid, lo - key0, hi - key0);
+                const float2 st = softmax_unit<C>(ts, sc, valid, rs);
                 sm.stats[i & 3][row] = st;
                 tmem_st_wait();
                 tc_fence_before();
