@@ -253,47 +253,53 @@ __device__ __forceinline__ long long line_of(const AttnParams &p, const AttnSeq 
 }
 
 // Query rows in, output rows out.
+// Elements i .. i + 15 as they are; those from n on are 0 (n a multiple of 8). The loads alone, so
+// that nothing waits between them; as f32 bits: widen16.
 template <int TYPE>
-__device__ __forceinline__ float load1(const void *q, size_t i) {
-    if constexpr (TYPE == JKB_F32) return __ldg(static_cast<const float *>(q) + i);
-    else if constexpr (TYPE == JKB_F16)
-        return __half2float(__ldg(static_cast<const __half *>(q) + i));
-    else return __bfloat162float(__ldg(static_cast<const __nv_bfloat16 *>(q) + i));
-}
-// Elements i .. i + 15 as f32 bits; those from n on are 0 (n a multiple of 8).
+struct Raw16 {
+    static constexpr int N = TYPE == JKB_F32 ? 16 : 8;
+    uint32_t w[N];
+};
 template <int TYPE>
-__device__ __forceinline__ void load16(const AttnParams &p, size_t i, int n, uint32_t (&x)[16]) {
+__device__ __forceinline__ void load16(const AttnParams &p, size_t i, int n, Raw16<TYPE> &x) {
+    constexpr int N = Raw16<TYPE>::N, PER = 16 / N;  // elements of a word
 #pragma unroll
-    for (int k = 0; k < 16; k++) x[k] = 0;
-    if (!p.q_vec) {
+    for (int k = 0; k < N; k++) x.w[k] = 0;
+    if (p.q_vec) {
+        const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const uint32_t *>(p.q) +
+                                                         i / PER);
 #pragma unroll
-        for (int k = 0; k < 16; k++)
-            if (k < n) x[k] = __float_as_uint(load1<TYPE>(p.q, i + k));
+        for (int k = 0; k < N / 4; k++)
+            if (4 * PER * k < n) {
+                const uint4 a = __ldg(q + k);
+                x.w[4 * k] = a.x, x.w[4 * k + 1] = a.y;
+                x.w[4 * k + 2] = a.z, x.w[4 * k + 3] = a.w;
+            }
         return;
     }
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        if (8 * h >= n) continue;
+    for (int k = 0; k < N; k++) {
+        if (PER * k >= n) continue;
         if constexpr (TYPE == JKB_F32) {
-            const uint4 *q = reinterpret_cast<const uint4 *>((const float *)p.q + i + 8 * h);
-            const uint4 a = __ldg(q), b = __ldg(q + 1);
-            x[8 * h] = a.x, x[8 * h + 1] = a.y, x[8 * h + 2] = a.z, x[8 * h + 3] = a.w;
-            x[8 * h + 4] = b.x, x[8 * h + 5] = b.y, x[8 * h + 6] = b.z, x[8 * h + 7] = b.w;
+            x.w[k] = __ldg(static_cast<const uint32_t *>(p.q) + i + k);
         } else {
-            const uint4 a =
-                __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)p.q + i + 8 * h));
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+            const uint16_t *q = static_cast<const uint16_t *>(p.q) + i + 2 * k;
+            x.w[k] = __ldg(q) | (uint32_t)__ldg(q + 1) << 16;
+        }
+    }
+}
+template <int TYPE>
+__device__ __forceinline__ void widen16(const Raw16<TYPE> &raw, uint32_t (&x)[16]) {
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if constexpr (TYPE == JKB_F16) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
-                    x[8 * h + 2 * k] = __float_as_uint(f.x);
-                    x[8 * h + 2 * k + 1] = __float_as_uint(f.y);
-                } else {
-                    x[8 * h + 2 * k] = w[k] << 16;
-                    x[8 * h + 2 * k + 1] = w[k] & 0xFFFF0000u;
-                }
-            }
+    for (int k = 0; k < Raw16<TYPE>::N; k++) {
+        const uint32_t w = raw.w[k];
+        if constexpr (TYPE == JKB_F32) {
+            x[k] = w;
+        } else if constexpr (TYPE == JKB_F16) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+            x[2 * k] = __float_as_uint(f.x), x[2 * k + 1] = __float_as_uint(f.y);
+        } else {
+            x[2 * k] = w << 16, x[2 * k + 1] = w & 0xFFFF0000u;
         }
     }
 }
@@ -546,16 +552,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         uint32_t it = 0;
         while (next_piece(ok)) {
             // ---- the query rows, 16 a warp: f16 parts of x times a power of two of the row ----
-            if (!wait(&sm.q_empty, pieces)) goto out;
-            // eight lanes a row, 16 dims a lane; two rounds of rows in flight
+            // eight lanes a row, 16 dims a lane; a round's rows are loaded before the one before
+            // is converted, the first before the tile before gives its place up
             {
                 const int d0 = 16 * (lane & 7);
                 int rr = cur.row0 + warp * 16 + (lane >> 3), tok = rr / p.group;
                 int h = rr - tok * p.group;
                 const size_t head0 = (size_t)(cur.head * p.group);
-#pragma unroll 1
-                for (int r0 = 0; r0 < 16; r0 += 4 * QROUNDS) {
-                    uint32_t x[QROUNDS][16];
+                auto load_round = [&](Raw16<C::TYPE>(&x)[QROUNDS]) {
 #pragma unroll
                     for (int j = 0; j < QROUNDS; j++) {
                         const size_t at = (size_t)(cur.q0 + tok) * p.q_token +
@@ -567,6 +571,16 @@ __global__ void __launch_bounds__(THREADS, 1)
                             tok++;
                         }
                     }
+                };
+                Raw16<C::TYPE> next[QROUNDS];
+                load_round(next);
+                if (!wait(&sm.q_empty, pieces)) goto out;
+#pragma unroll 1
+                for (int r0 = 0; r0 < 16; r0 += 4 * QROUNDS) {
+                    uint32_t x[QROUNDS][16];
+#pragma unroll
+                    for (int j = 0; j < QROUNDS; j++) widen16<C::TYPE>(next[j], x[j]);
+                    if (r0 + 4 * QROUNDS < 16) load_round(next);
 #pragma unroll
                     for (int j = 0; j < QROUNDS; j++) {
                         const int r = warp * 16 + r0 + 4 * j + (lane >> 3);
