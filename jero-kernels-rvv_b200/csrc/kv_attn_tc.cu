@@ -44,7 +44,7 @@
 // Measured, 32 query heads over 8 kv heads of 128 dims: a causal prompt of 2048 f32 tokens behind
 // 1111 cached ones takes 213 us (337 TFLOP/s of its two products; the 5 f16 products that f32
 // needs run at 840), one of 8192 bf16 tokens 997 us (551 TFLOP/s; with p's second part 827; 904
-// us where the clock is not held back by power); nine ragged f16 chunks, 5331 tokens of 14 query
+// us before the power limit lowers the clock); nine ragged f16 chunks, 5331 tokens of 14 query
 // heads over 2 of 80 dims, 154 us. What bounds a unit are the issue slots above; a tile's start
 // and end cost as much as 5 units.
 #include "kv_attn.cuh"
