@@ -198,8 +198,11 @@ __device__ __forceinline__ float finite_or_0(float v) { return isfinite(v) ? v :
 
 // Code of one element in the low byte: rint(x * inv), ties to even; |x * inv| < 127.5, and adding
 // 1.5 * 2^23 rounds to an integer, whose two's complement the low bits are.
-__device__ __forceinline__ uint32_t code_of(float x, float inv) {
-    return __float_as_uint(__fadd_rn(__fmul_rn(finite_or_0(x), inv), 12582912.0f));
+__device__ __forceinline__ uint32_t code_of(float x, float inv) {  // x finite
+    return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f));
+}
+__device__ __forceinline__ float4 finite_or_0(float4 v) {
+    return make_float4(finite_or_0(v.x), finite_or_0(v.y), finite_or_0(v.z), finite_or_0(v.w));
 }
 // The low bytes of four words.
 __device__ __forceinline__ uint32_t low4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -240,9 +243,14 @@ __device__ __forceinline__ void append_run(const Run &r, const AppendSide &src, 
     const float old = r.o ? *scale : 0.0f;
     const int quads = dim >> 2;
     float amax = 0.0f;
+    bool odd = false;  // an element that is not finite
     {
         int t = tid / quads, q = tid - t * quads;
         const int step_t = team / quads, step_q = team - step_t * quads;
+        size_t at = row0 + t * src.token_stride + 4 * q;
+        const size_t step = step_t * src.token_stride + 4 * step_q;
+        const size_t wrap = src.token_stride - 4 * quads;
+        float zero = 0.0f;  // NaN once an element is not finite
 #pragma unroll 1
         while (t < r.n) {
             constexpr int U = VEC ? 8 : 2;  // loads in flight
@@ -250,33 +258,45 @@ __device__ __forceinline__ void append_run(const Run &r, const AppendSide &src, 
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (t < r.n)
-                    v[u] = elem4<TYPE, VEC>(src.data, row0 + t * src.token_stride + 4 * q);
+                if (t < r.n) v[u] = elem4<TYPE, VEC>(src.data, at);
                 t += step_t;
                 q += step_q;
+                at += step;
                 if (q >= quads) {
                     q -= quads;
                     t++;
+                    at += wrap;
                 }
             }
 #pragma unroll
-            for (int u = 0; u < U; u++)  // (fmaxf passes over a NaN)
+            for (int u = 0; u < U; u++) {  // (fmaxf passes over a NaN)
                 amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v[u].x), fabsf(v[u].y)),
                                          fmaxf(fabsf(v[u].z), fabsf(v[u].w))));
+                zero = fmaf(v[u].x, 0.f, fmaf(v[u].y, 0.f, zero));
+                zero = fmaf(v[u].z, 0.f, fmaf(v[u].w, 0.f, zero));
+            }
         }
+        odd = !(zero == 0.0f);
         if (amax == INFINITY) {  // infinities count as 0: once more without them
             amax = 0.0f;
 #pragma unroll 1
-            for (int i = tid; i < r.n * dim; i += team)
-                amax = fmaxf(amax, fabsf(finite_or_0(elem<TYPE>(
-                                       src.data, row0 + i / dim * src.token_stride + i % dim))));
+            for (int i = tid; i < r.n * quads; i += team) {
+                const float4 v = finite_or_0(elem4<TYPE, VEC>(
+                    src.data, row0 + i / quads * src.token_stride + 4 * (i % quads)));
+                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)),
+                                         fmaxf(fabsf(v.z), fabsf(v.w))));
+            }
         }
     }
     for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, d));
-    if (team > 32) {
-        if ((tid & 31) == 0) red[tid >> 5] = amax;
+    odd = __any_sync(~0u, odd);
+    if (team > 32) {  // (a warp's sign: odd)
+        if ((tid & 31) == 0) red[tid >> 5] = odd ? -amax : amax;
         __syncthreads();
-        for (int w = 0; w < APPEND_THREADS / 32; w++) amax = fmaxf(amax, red[w]);
+        for (int w = 0; w < APPEND_THREADS / 32; w++) {
+            odd |= (__float_as_uint(red[w]) >> 31) != 0;
+            amax = fmaxf(amax, fabsf(red[w]));
+        }
         __syncthreads();
     } else {
         __syncwarp();
@@ -294,43 +314,78 @@ __device__ __forceinline__ void append_run(const Run &r, const AppendSide &src, 
     // the groups that are new as a whole
     const int f0 = (r.o + KV_GROUP - 1) / KV_GROUP, f1 = max(f0, end / KV_GROUP);
     const int per = dim_p >> 4;  // key patches of a token
+    const int n_new = (f1 - f0) * patches;
+    const size_t row_f0 = row0 + (size_t)(f0 * KV_GROUP - r.o) * src.token_stride;
+    uint8_t *page_f0 = page + (size_t)f0 * 32 * dim_p;
+    if (!value) {
+        int tok = tid / per, c16 = tid - tok * per;
+        const int step_t = team / per, step_c = team - step_t * per;
 #pragma unroll 1
-    for (int i = tid; i < (f1 - f0) * patches; i += team) {
-        // v[k]: dims d0 + 4 k .. of token tok, or dims d0 .. of token tok + (k & 1) + 8 (k >> 1)
-        int tok, d0;
-        uint8_t *at;
-        size_t step[2];
-        if (!value) {
-            tok = i / per;
-            d0 = 16 * (i - tok * per);
-            at = page + (size_t)(f0 + (tok / KV_GROUP)) * 32 * dim_p +
-                 kv_key_at(tok % KV_GROUP, d0, dim_p);
-            step[0] = 4, step[1] = 8;
-        } else {
-            const int chunks = i >> 5, q8 = i & 31, tt = q8 >> 3;  // chunks: of 32 dims
-            const int grp = chunks / (dim_p >> 5), chunk = chunks - grp * (dim_p >> 5);
-            tok = grp * KV_GROUP + 2 * tt;
-            d0 = 32 * chunk + 4 * ((q8 & 7) ^ (2 * tt));
-            at = page + (size_t)(f0 + grp) * 32 * dim_p + 16 * dim_p + 512 * chunk + 16 * q8;
-            step[0] = src.token_stride, step[1] = 8 * src.token_stride;
-        }
-        const size_t row = row0 + (size_t)(f0 * KV_GROUP + tok - r.o) * src.token_stride + d0;
-        uint32_t c[4][4];
+        for (int i = tid; i < n_new; i += team) {
+            const size_t row = row_f0 + tok * src.token_stride + 16 * c16;
+            float4 v[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if ((value ? d0 : d0 + 4 * k) < dim)
-                v = elem4<TYPE, VEC>(src.data,
-                                     row + (k & 1 ? step[0] : 0) + (k >> 1 ? step[1] : 0));
-            c[k][0] = code_of(v.x, inv), c[k][1] = code_of(v.y, inv);
-            c[k][2] = code_of(v.z, inv), c[k][3] = code_of(v.w, inv);
-        }
-        uint32_t w[4];
+            for (int k = 0; k < 4; k++) {
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (16 * c16 + 4 * k < dim) v[k] = elem4<TYPE, VEC>(src.data, row + 4 * k);
+            }
+            if (odd)
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-            w[k] = value ? 0x80808080u ^ low4(c[0][k], c[1][k], c[2][k], c[3][k])
-                         : low4(c[k][0], c[k][1], c[k][2], c[k][3]);
-        *reinterpret_cast<uint4 *>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int k = 0; k < 4; k++) v[k] = finite_or_0(v[k]);
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                w[k] = low4(code_of(v[k].x, inv), code_of(v[k].y, inv), code_of(v[k].z, inv),
+                            code_of(v[k].w, inv));
+            *reinterpret_cast<uint4 *>(page_f0 + (size_t)(tok / KV_GROUP) * 32 * dim_p +
+                                       kv_key_at(tok % KV_GROUP, 16 * c16, dim_p)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+            tok += step_t;
+            c16 += step_c;
+            if (c16 >= per) {
+                c16 -= per;
+                tok++;
+            }
+        }
+    } else {
+        const int q8 = tid & 31, tt = q8 >> 3, chunks = dim_p >> 5;  // chunks: of 32 dims
+        int grp = (tid >> 5) / chunks, chunk = (tid >> 5) - grp * chunks;
+        const int d_lane = 4 * ((q8 & 7) ^ (2 * tt));
+        const size_t lane_row = row_f0 + 2 * tt * src.token_stride + d_lane;
+#pragma unroll 1
+        for (int i = tid; i < n_new; i += team) {
+            const size_t row = lane_row + (size_t)(grp * KV_GROUP) * src.token_stride + 32 * chunk;
+            const bool on = 32 * chunk + d_lane < dim;
+            float4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (on)
+                    v[k] = elem4<TYPE, VEC>(
+                        src.data, row + (size_t)((k & 1) + 8 * (k >> 1)) * src.token_stride);
+            }
+            if (odd)
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = finite_or_0(v[k]);
+            uint32_t c[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                c[k][0] = code_of(v[k].x, inv), c[k][1] = code_of(v[k].y, inv);
+                c[k][2] = code_of(v[k].z, inv), c[k][3] = code_of(v[k].w, inv);
+            }
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                w[j] = 0x80808080u ^ low4(c[0][j], c[1][j], c[2][j], c[3][j]);
+            *reinterpret_cast<uint4 *>(page_f0 + (size_t)grp * 32 * dim_p + 16 * dim_p +
+                                       512 * chunk + 16 * q8) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+            chunk += team >> 5;
+            while (chunk >= chunks) {
+                chunk -= chunks;
+                grp++;
+            }
+        }
     }
     // the groups before and after, which keep bytes or end within
     const int before = max(f0 - g0, 0) * patches, after = (g1 - f1) * patches;
@@ -353,7 +408,7 @@ __device__ __forceinline__ void append_run(const Run &r, const AppendSide &src, 
                     w = pack4(recode<false>(x, 0, ratio), recode<false>(x, 1, ratio),
                               recode<false>(x, 2, ratio), recode<false>(x, 3, ratio));
                 } else if (d0 + 4 * k < dim) {
-                    const float4 v = elem4<TYPE, VEC>(src.data, row + 4 * k);
+                    const float4 v = finite_or_0(elem4<TYPE, VEC>(src.data, row + 4 * k));
                     w = low4(code_of(v.x, inv), code_of(v.y, inv), code_of(v.z, inv),
                              code_of(v.w, inv));
                 }
@@ -376,8 +431,8 @@ __device__ __forceinline__ void append_run(const Run &r, const AppendSide &src, 
                 if (is_new) {
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (d0 < dim)
-                        v = elem4<TYPE, VEC>(src.data,
-                                             row0 + (size_t)(off - r.o) * src.token_stride + d0);
+                        v = finite_or_0(elem4<TYPE, VEC>(
+                            src.data, row0 + (size_t)(off - r.o) * src.token_stride + d0));
                     c[0] = code_of(v.x, inv) + 128, c[1] = code_of(v.y, inv) + 128;
                     c[2] = code_of(v.z, inv) + 128, c[3] = code_of(v.w, inv) + 128;
                 } else {
