@@ -231,7 +231,7 @@ struct Run {
 // Instructions bound it, their number an element and, as each runs a few times a run, their
 // fetching: the rare paths are loops over little code. (Patches kept in registers between the
 // passes, in eight times the code, took twice as long.) 5985 f32 tokens of 8 heads of 128 take 23
-// us (2.6 TB/s of rows and codes), 16,411 bf16 tokens 45 us (2.3 TB/s), 24 single tokens 8 us.
+// us (2.6 TB/s of rows and codes), 16,411 bf16 tokens 40 us (2.5 TB/s), 24 single tokens 8 us.
 template <int TYPE, bool VEC>
 __device__ __forceinline__ void append_run(const Run &r, const AppendSide &src, bool value,
                                            int head, int tid, int team, uint8_t *codes,
