@@ -796,7 +796,9 @@ int jkb_attn_workspace_destroy(jkb_attn_workspace *ws);
  * keys and values of kv head h / (n_heads / n_kv_heads); lse[t][h] = log sum_j exp(s_j). A query
  * that sees no token has out = 0 and lse = -inf; one with a non-finite element has NaN.
  * q and out share a type; out rows may be strided too. Sums, softmax statistics and the
- * accumulated output are f32 for every type. max_new: an upper bound of the query tokens of a
+ * accumulated output are f32 for every type. A weight enters its product with v in 22 bits in the
+ * few-row kernel, in the prompt kernel in 24 bits for f32 rows and in 16 for f16 and bf16 rows; lse
+ * does not take part in that rounding. max_new: an upper bound of the query tokens of a
  * sequence (it selects the kernels; outputs stay right above it, but slow). Sequences of up to 16
  * query rows (tokens times n_heads / n_kv_heads), and all of head_dim > 128, take the few-row
  * kernel, where a token whose weight is below 2^-39 of its row's largest counts as 0; the others

@@ -8,9 +8,10 @@
 //                       f32 rows as two f16, 22 bits), K the codes, exact in f16
 //   s = c ks S,  m = max s,  p = 2^(s - m),  l = sum p          (of the unit alone)
 //   o = a o + b (p vs) V,  l' = a l' + b l,  m' = max(m', m),  a, b = 2^(old m' - m'), 2^(m - m')
-//                       V the codes, exact in f16 and bf16; p vs in f16 (f16 rows), in two bf16
-//                       (bf16 rows) or three (f32 rows). bf16 has f32's range: a weight that is
-//                       far below its row's largest keeps its digits.
+//                       V the codes, exact in bf16; p vs in two bf16 (16-bit rows: 16 bits, five
+//                       more than an f16 output has) or three (f32 rows: 24). bf16 has f32's
+//                       range: a weight that is far below its row's largest keeps its digits, and
+//                       so do the weights beside a block whose value scale is far above theirs.
 // The tensor core truncates its f32 sums, about 2^-25 of the sum at every 16-element step. So S
 // takes the small part of Q first, and each unit's P V starts from zero, small parts first, and
 // is added to o in registers, rounded, with the rescale.
@@ -23,7 +24,7 @@
 //   0, 1  the query rows of a new tile; softmax, every other unit each (a unit's needs nothing of
 //         the one before): a thread a row; S from TMEM, p's parts back over it
 //   2     accumulation: a thread a row; the unit's P V from TMEM, o in registers; the output
-//   3, 4  conversion of keys, of values: codes from the raw rings to f16 / bf16 operand tiles
+//   3, 4  conversion of keys (f16), of values (bf16): codes from the raw rings to operand tiles
 //         (128-byte swizzle)
 //   5     a warp that issues the MMAs, one that loads keys and one that loads values (a bulk copy
 //         for 16 tokens each, kv_cache.cuh), and one that finds this CTA's pieces of tiles and
@@ -45,7 +46,8 @@
 // 1111 cached ones takes 213 us (337 TFLOP/s of its two products; the 5 f16 products that f32
 // needs run at 840), one of 8192 bf16 tokens 997 us (551 TFLOP/s; with p's second part 827; 904
 // us before the power limit lowers the clock); nine ragged f16 chunks, 5331 tokens of 14 query
-// heads over 2 of 80 dims, 154 us. What bounds a unit are the issue slots above; a tile's start
+// heads over 2 of 80 dims, 166 us (155 with p in one f16 part, 11 bits, whose error is as large as
+// the output's rounding). What bounds a unit are the issue slots above; a tile's start
 // and end cost as much as 5 units.
 #include "kv_attn.cuh"
 #include "ptx.cuh"
@@ -74,14 +76,12 @@ static_assert(REGS_SOFT >= REGS_LAUNCH && REGS_SUM >= REGS_LAUNCH && REGS_CONV <
                   REGS_REST <= REGS_LAUNCH,
               "an increase must not go down, nor a decrease up: either is an illegal instruction");
 
-// TYPE: the rows'. NQ: f16 parts of a query element; NP: parts of p; F16: p and V are f16 (else
-// bf16).
+// TYPE: the rows'. NQ: f16 parts of a query element; NP: bf16 parts of p.
 template <int DT_, int TYPE_>
 struct PreCfg {
     static constexpr int DT = DT_, TYPE = TYPE_;
-    static constexpr bool F16 = TYPE == JKB_F16;
     static constexpr int NQ = TYPE == JKB_F32 ? 2 : 1;
-    static constexpr int NP = TYPE == JKB_F32 ? 3 : TYPE == JKB_BF16 ? 2 : 1;
+    static constexpr int NP = TYPE == JKB_F32 ? 3 : 2;
     static constexpr int DIM = 32 * DT;
     static constexpr int KA = (DIM + 63) / 64;       // 64-element swizzle atoms of a head
     static constexpr int NV = NQ == 2 ? 1 : 2;       // V buffers
@@ -341,22 +341,6 @@ __device__ __forceinline__ void store8(const AttnParams &p, size_t i, const floa
     }
 }
 
-// f16 p: the unit's largest value scale is below 2^vexp, and vs enters as vs 2^(14 - vexp).
-__device__ __forceinline__ int unit_vexp(const float2 *sc, uint32_t valid) {
-    int e = -126;
-#pragma unroll
-    for (int g = 0; g < GROUPS; g++)
-        if ((valid >> g) & 1)
-            e = max(e, (int)((__float_as_uint(sc[g].y) >> 23) & 255) - 126);
-    return e;
-}
-__device__ __forceinline__ float scale_f16(float vs, int vexp) {
-    const uint32_t b = __float_as_uint(vs);
-    return (b & 0x7F800000u) ? __uint_as_float((b & 0x807FFFFFu) | 0x3F000000u) *
-                                   ex2((float)((int)((b >> 23) & 255) - 126 - vexp + 14))
-                             : 0.0f;
-}
-
 // Tokens outside lo .. hi of the unit, and of groups that are not there, get S = -inf, before
 // softmax_unit, which so needs no test for them: beside a second form of it with the tests, which
 // a tile's last units ran from a cold instruction cache, this took 5 to 9 us less a tile.
@@ -392,8 +376,7 @@ __device__ __forceinline__ void mask_unit(uint32_t ts, uint32_t valid, int lo, i
 // rs and ks are not negative (a negative softmax scale's sign is in Q); where they give 0, the
 // smallest normal number in its place keeps a masked token's -inf.
 template <class C>
-__device__ __forceinline__ float2 softmax_unit(uint32_t ts, const float2 *sc, uint32_t valid,
-                                               float rs) {
+__device__ __forceinline__ float2 softmax_unit(uint32_t ts, const float2 *sc, float rs) {
     constexpr int NP = C::NP;
     float top = -INFINITY, most = -INFINITY;  // of s; of S
     uint32_t r[32];
@@ -418,8 +401,6 @@ __device__ __forceinline__ float2 softmax_unit(uint32_t ts, const float2 *sc, ui
     }
     const float ref = top == -INFINITY ? 0.0f : top;
     if (most == -INFINITY) rs = 0.0f;  // sees nothing here: no NaN from its scale either
-    int vexp = 0;
-    if (C::F16) vexp = unit_vexp(sc, valid);
     const uint64_t nref = pkf(-ref, -ref), minus = pkf(-1.0f, -1.0f);
     uint64_t sum = 0;
 #pragma unroll 1
@@ -430,7 +411,7 @@ __device__ __forceinline__ float2 softmax_unit(uint32_t ts, const float2 *sc, ui
             const int g = 2 * h + k;
             float f = rs * sc[g].x;
             f = f < FLT_MIN ? FLT_MIN : f;
-            const float vs = C::F16 ? scale_f16(sc[g].y, vexp) : sc[g].y;
+            const float vs = sc[g].y;
             uint32_t part[NP][8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -440,24 +421,19 @@ __device__ __forceinline__ float2 softmax_unit(uint32_t ts, const float2 *sc, ui
                 sum = add2(sum, e);
                 e = mul2(e, pkf(vs, vs));
                 upk2(e, u, w);
-                if (C::F16) {
-                    const __half2 y = __floats2half2_rn(u, w);
-                    part[0][i] = *reinterpret_cast<const uint32_t *>(&y);
-                } else {
-                    // all parts but the last are cut off, not rounded: the upper halves
+                // all parts but the last are cut off, not rounded: the upper halves
 #pragma unroll
-                    for (int j = 0; j < NP - 1; j++) {
-                        const uint32_t a = __float_as_uint(u), b = __float_as_uint(w);
-                        part[j][i] = __byte_perm(a, b, 0x7632);
-                        e = fma2(pk2(a & 0xFFFF0000u, b & 0xFFFF0000u), minus, e);
-                        upk2(e, u, w);
-                    }
-                    const __nv_bfloat162 y = __floats2bfloat162_rn(u, w);
-                    part[NP - 1][i] = *reinterpret_cast<const uint32_t *>(&y);
+                for (int j = 0; j < NP - 1; j++) {
+                    const uint32_t a = __float_as_uint(u), b = __float_as_uint(w);
+                    part[j][i] = __byte_perm(a, b, 0x7632);
+                    e = fma2(pk2(a & 0xFFFF0000u, b & 0xFFFF0000u), minus, e);
+                    upk2(e, u, w);
                 }
+                const __nv_bfloat162 y = __floats2bfloat162_rn(u, w);
+                part[NP - 1][i] = *reinterpret_cast<const uint32_t *>(&y);
             }
             tmem_st8(ts + 16 * g, part[0]);
-            if (NP > 1) tmem_st8(ts + 16 * g + 8, part[NP > 1 ? 1 : 0]);
+            tmem_st8(ts + 16 * g + 8, part[1]);
             if (NP > 2) tmem_st8(ts + TN + 8 * g, part[NP - 1]);
         }
         if (h < 3) tmem_ld32(ts + 32 * (h + 1), r);
@@ -648,7 +624,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const uint32_t ts = tl + b * C::S_COLS;
                 if (key0 < cur.all_lo || key0 + TN > cur.all_hi || valid != 0xFFu)
                     mask_unit(ts, valid, lo - key0, hi - key0);
-                const float2 st = softmax_unit<C>(ts, sc, valid, rs);
+                const float2 st = softmax_unit<C>(ts, sc, rs);
                 sm.stats[i & 3][row] = st;
                 tmem_st_wait();
                 tc_fence_before();
@@ -676,9 +652,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 l = fmaf(l, a, b * st.y);
                 m = mn;
                 const uint64_t a2 = pkf(a, a);
-                float up = b;  // f16 (a power of two that flushes to 0 is below f16's smallest)
-                if (C::F16) up *= ex2((float)(unit_vexp(sm.sc[it % SC], sm.valid[it % SC]) - 14));
-                const uint64_t b2 = pkf(up, up);
+                const uint64_t b2 = pkf(b, b);
 #pragma unroll
                 for (int q = 0; q < DT; q++) {
                     uint32_t r[32];
@@ -888,8 +862,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                             uint32_t y[4];
 #pragma unroll
                             for (int t = 0; t < 4; t++)
-                                y[t] = C::F16 ? pair_f16(w[t][j], i ? 0x4342 : 0x4140)
-                                              : pair_bf16(w[t][j], i);
+                                y[t] = pair_bf16(w[t][j], i);
                             *reinterpret_cast<uint4 *>(dst + j * 8 * 128 + (d0 ^ (16 * i))) =
                                 make_uint4(y[0], y[1], y[2], y[3]);
                         }
@@ -905,7 +878,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
     } else if (warp == 20) {
         // ------------------------------------------------------------ MMA
-        constexpr uint32_t ID_S = idesc_f16(TN, false), ID_O = idesc_f16(DIM, !C::F16);
+        constexpr uint32_t ID_S = idesc_f16(TN, false), ID_O = idesc_f16(DIM, true);
         uint32_t it = 0, pv = 0;  // S and P V issued so far
         const uint32_t ut = uniform(tmem), vd0 = uniform(desc_lo(&sm.v[0][0][0]));
         const uint32_t kd = uniform(desc_lo(&sm.k[0][0])), qd = uniform(desc_lo(&sm.q[0][0][0]));
