@@ -200,9 +200,11 @@ __device__ __forceinline__ void store4(const AttnParams &p, int type, size_t i, 
 }
 
 // A query row is held as integers |n| < 127 * (65536 + 256 + 1) in three signed base-256 digits,
-// x = unit * n: the bytes of (n + 0x808080) ^ 0x808080. MOST leaves room for the rounding of
-// x / unit. A row with a non-finite element has unit NaN, so that its output is NaN; below 1e-30
-// the row counts as 0 (its scores are 0 to f32's accuracy).
+// x = unit / 65536 * n: the bytes of (n + 0x808080) ^ 0x808080. MOST leaves room for the rounding of
+// n. A power of two brings the row's largest element near 1 before MOST is divided by it, so that
+// rows of any finite size have their 24 bits; the 65536, which the scores put back, keeps unit a
+// normal number for rows down to 2^-119 / scale (below, it has fewer bits). A row with a non-finite
+// element has unit NaN, so that its output is NaN.
 constexpr float MOST = 8355700.0f;
 
 // Units of one sequence and its row tiles.
@@ -429,16 +431,17 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
                 top = __reduce_max_sync(~0u, top);
                 const bool finite = top < 0x7F800000u;
                 const float amax = __uint_as_float(top);
-                const float inv = finite && amax > 1e-30f ? __fdividef(MOST, amax) : 0.0f;
+                const float up = __uint_as_float(min(255 - (top >> 23), 254u) << 23);
+                const float inv = finite && top ? __fdividef(MOST, amax * up) : 0.0f;
 #pragma unroll
                 for (int k = 0; k < DL; k++) {
                     const int d = 128 * k + 4 * lane;
                     if (DIM % 128 && d >= DIM) break;
                     uint32_t w[4];
-                    w[0] = (uint32_t)(__float2int_rn(x[k].x * inv) + 0x808080) ^ 0x808080u;
-                    w[1] = (uint32_t)(__float2int_rn(x[k].y * inv) + 0x808080) ^ 0x808080u;
-                    w[2] = (uint32_t)(__float2int_rn(x[k].z * inv) + 0x808080) ^ 0x808080u;
-                    w[3] = (uint32_t)(__float2int_rn(x[k].w * inv) + 0x808080) ^ 0x808080u;
+                    w[0] = (uint32_t)(__float2int_rn(x[k].x * up * inv) + 0x808080) ^ 0x808080u;
+                    w[1] = (uint32_t)(__float2int_rn(x[k].y * up * inv) + 0x808080) ^ 0x808080u;
+                    w[2] = (uint32_t)(__float2int_rn(x[k].z * up * inv) + 0x808080) ^ 0x808080u;
+                    w[3] = (uint32_t)(__float2int_rn(x[k].w * up * inv) + 0x808080) ^ 0x808080u;
                     const uint32_t a = __byte_perm(w[0], w[1], 0x5140);
                     const uint32_t b = __byte_perm(w[2], w[3], 0x5140);
                     *reinterpret_cast<uint32_t *>(&sm.digits[r][2][d]) =
@@ -449,9 +452,12 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
                         __byte_perm(__byte_perm(w[0], w[1], 0x0062),
                                     __byte_perm(w[2], w[3], 0x0062), 0x5410);
                 }
-                if (lane == 0)
-                    sm.unit[r] =
-                        (finite ? amax / MOST : __int_as_float(0x7FC00000)) * p.scale2;
+                if (lane == 0) {
+                    constexpr float C65536 = 65536.0f / MOST;
+                    sm.unit[r] = !finite       ? __int_as_float(0x7FC00000)
+                                 : amax > 1.0f ? amax * C65536 * p.scale2
+                                               : amax * (C65536 * p.scale2);
+                }
             }
             __syncthreads();
 #pragma unroll
@@ -532,7 +538,7 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
                         const int d1 = RH == 1 ? a[0][2 + e] : a[1][2 * r + e];
                         const int d2 = RH == 1 ? a[2][e] : a[2][2 * r + e];
                         sc[r][4 * i + k] =
-                            fmaf((float)d0, 65536.0f, fmaf((float)d1, 256.0f, (float)d2)) * f_row;
+                            fmaf((float)(d1 * 256 + d2), 1.0f / 65536.0f, (float)d0) * f_row;
                     }
                 }
             if (f.t0 < all_lo || f.t0 + C::STEP > all_hi || (G > 1 && !(f.src[0] && f.src[G - 1]))) {
