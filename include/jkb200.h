@@ -801,8 +801,8 @@ int jkb_attn_workspace_destroy(jkb_attn_workspace *ws);
  * does not take part in that rounding. max_new: an upper bound of the query tokens of a
  * sequence (it selects the kernels; outputs stay right above it, but slow). Sequences of up to 16
  * query rows (tokens times n_heads / n_kv_heads), and all of head_dim > 128, take the few-row
- * kernel, where a token whose weight is below 2^-39 of its row's largest counts as 0; the others
- * take the prompt kernel. Results do not depend on timing: a call repeated gives the same bits. */
+ * kernel, where a token whose weight times its block's value scale is below 2^-37 of the largest
+ * such product of its row counts as 0; the others take the prompt kernel. Results do not depend on timing: a call repeated gives the same bits. */
 typedef struct {
     const jkb_kv_cache *cache;
     jkb_attn_workspace *ws;

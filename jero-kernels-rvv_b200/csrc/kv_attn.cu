@@ -14,10 +14,13 @@
 //     tile takes a row's second digit. (Two digits, 16 bits, would do for a 16-bit output but not
 //     for its f32 lse: 1e-5 off.)
 //   * p v runs as mma.m16n8k16 on f16: p, times the block's value scale relative to a power of
-//     two, is split into two f16 (22 bits; the second in the A tile's lower half), the codes are
-//     exact in f16. The tensor core truncates its sums, so each step starts from zero and is
-//     added to o in f32 on the FMA pipe, together with the rescale. (A weight below 2^-39 of its
-//     row's largest falls out of f16's range and counts as 0.)
+//     two of the row's, is split into two f16 (22 bits; the second in the A tile's lower half), the
+//     codes are exact in f16. The tensor core truncates its sums, so each step starts from zero and
+//     is added to o in f32 on the FMA pipe, together with the rescale. m is rounded up to a whole
+//     number, and the row's power of two, 2^big, is that of the largest p vs among the tokens that
+//     the row has seen, so both rescales are exact. (A p vs below 2^-37 of the row's largest falls
+//     out of f16's range and counts as 0; a block that a row does not see, or gives no weight,
+//     takes nothing from the others, whatever its scale.)
 //
 // A step of one warp is G groups of 16 tokens (kv_cache.cuh), each one bulk copy into the warp's
 // ring, issued by the warp itself three steps ahead. Two groups share a step's softmax and its o
@@ -372,10 +375,10 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
     // ---- running state of the current row tile ----
     uint32_t qa[ND][DT][2 * RH];  // A registers of each digit
     float m[RH], l[RH], unit[RH];
+    float big[RH];  // o is in units of 2^(big - 14)
     int lo[RH], hi[RH], all_lo = 0, all_hi = 0;  // tokens that the rows see; that all see
     uint64_t o[RH][DT][4];  // pairs: dims 32 c + 8 tg + j and + 4 + j of row g (+ 8)
-    int vexp = 0;
-    bool seen = false, dead = false;
+    bool dead = false;
     uint32_t phases = 0;
 
     Look look = find(0);
@@ -477,14 +480,13 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
                 const int pos = q.len - q.nq + tok;
                 hi[r] = !on ? 0 : p.causal ? min(q.len, pos + 1) : q.len;
                 lo[r] = p.window ? max(0, pos - p.window + 1) : 0;
-                m[r] = -INFINITY;
+                m[r] = big[r] = -INFINITY;
                 l[r] = 0.0f;
 #pragma unroll
                 for (int c = 0; c < DT; c++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) o[r][c][i] = 0;
             }
-            seen = false;
             const int last = min((tile + 1) * ROWS, q.nq * p.group) - 1;  // of the tile's rows
             const int pos_a = q.len - q.nq + tile * ROWS / p.group;
             const int pos_b = q.len - q.nq + last / p.group;
@@ -550,53 +552,53 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
                         if (t < lo[r] || t >= hi[r] || !f.src[k / 4]) sc[r][k] = -INFINITY;
                     }
             }
-            // ---- the blocks' value scales relative to a power of two: vs = mant * 2^e ----
-            float vmul[G], shift = 1.0f;
-            int e[G], most = INT_MIN;
+            // ---- the blocks' value scales: vs = mant * 2^e ----
+            float mant[G], e[G];
 #pragma unroll
             for (int i = 0; i < G; i++) {
                 const uint32_t vb = __float_as_uint(f.sc[i].y);
-                e[i] = (int)((vb >> 23) & 255) - 126;
-                vmul[i] = (vb & 0x7F800000u) ? __uint_as_float((vb & 0x807FFFFFu) | 0x3F000000u)
+                e[i] = (float)((int)((vb >> 23) & 255) - 126);
+                mant[i] = (vb & 0x7F800000u) ? __uint_as_float((vb & 0x807FFFFFu) | 0x3F000000u)
                                              : 0.0f;
-                if (f.src[i]) most = max(most, e[i]);
             }
-            if (!seen) {
-                vexp = most;
-                seen = true;
-            } else if (most > vexp) {
-                shift = ex2((float)(vexp - most));
-                vexp = most;
-            }
-#pragma unroll
-            for (int i = 0; i < G; i++)
-                vmul[i] = f.src[i] ? vmul[i] * ex2((float)(e[i] - vexp + 14)) : 0.0f;
             // ---- softmax step ----
             uint32_t ph[RH][G][2], pl[RH][G][2];
             uint64_t alpha[RH];
 #pragma unroll
             for (int r = 0; r < RH; r++) {
-                float top = fmaxf(fmaxf(sc[r][0], sc[r][1]), fmaxf(sc[r][2], sc[r][3]));
+                float top[G], mn = m[r];
 #pragma unroll
-                for (int k = 4; k < 4 * G; k++) top = fmaxf(top, sc[r][k]);
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                const float mn = fmaxf(m[r], top);
+                for (int i = 0; i < G; i++) {
+                    const float *x = sc[r] + 4 * i;
+                    top[i] = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 1));
+                    top[i] = ceilf(fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 2)));
+                    mn = fmaxf(mn, top[i]);
+                }
                 const float ref = mn == -INFINITY ? 0.0f : mn;
                 const float a = ex2(m[r] - ref);
                 m[r] = mn;
+                float bn = big[r];
+#pragma unroll
+                for (int i = 0; i < G; i++)  // (weights below 2^-112 count as 0)
+                    if (top[i] >= ref - 112.0f) bn = fmaxf(bn, top[i] + e[i]);
+                const float bref = bn == -INFINITY ? 0.0f : bn, shift = ex2(big[r] - bref);
+                big[r] = bn;
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < G; i++) {
+                    // at most 2^126, where the weights are below 2^-112
+                    const float vmul =
+                        top[i] >= ref - 112.0f ? mant[i] * ex2(ref - bref + e[i] + 14.0f) : 0.0f;
                     float w[4];
 #pragma unroll
                     for (int k = 0; k < 4; k++) w[k] = ex2(sc[r][4 * i + k] - ref);
                     sum += (w[0] + w[1]) + (w[2] + w[3]);
-                    split_f16(w[0] * vmul[i], w[1] * vmul[i], ph[r][i][0], pl[r][i][0]);
-                    split_f16(w[2] * vmul[i], w[3] * vmul[i], ph[r][i][1], pl[r][i][1]);
+                    split_f16(w[0] * vmul, w[1] * vmul, ph[r][i][0], pl[r][i][0]);
+                    split_f16(w[2] * vmul, w[3] * vmul, ph[r][i][1], pl[r][i][1]);
                 }
                 l[r] = fmaf(l[r], a, sum);
-                alpha[r] = pkf(a * shift, a * shift);
+                alpha[r] = pkf(shift, shift);
             }
             // ---- o = o * alpha + p v ----
 #pragma unroll
@@ -679,13 +681,13 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
         }
         __syncthreads();
         float mul[RH];
-        const float pow2 = seen ? ldexpf(1.0f, vexp - 14) : 1.0f;
 #pragma unroll
         for (int r = 0; r < RH; r++) {
             float top = -INFINITY;
             for (int w = 0; w < NW; w++) top = fmaxf(top, sm.row_m[w][g + 8 * r]);
-            mul[r] = ex2(m[r] - (top == -INFINITY ? 0.0f : top));
-            if (tg == 0) sm.row_l[warp][g + 8 * r] *= mul[r];
+            if (top == -INFINITY) top = 0.0f;
+            if (tg == 0) sm.row_l[warp][g + 8 * r] *= ex2(m[r] - top);
+            mul[r] = ex2(big[r] - 14.0f - top);
         }
         // where this piece's sums go: the output, or its slot in the workspace
         const bool whole = flags & STEP_WHOLE;
@@ -727,7 +729,7 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
                             for (int j = 0; j < 4; j++) {
                                 float u, w;
                                 upk2(o[r][c][j], u, w);
-                                x[j] = (k ? w : u) * mul[r] * pow2;
+                                x[j] = (k ? w : u) * mul[r];
                             }
                             const float4 v = make_float4(x[0], x[1], x[2], x[3]);
                             *reinterpret_cast<float4 *>(&sm.merge[warp][g + 8 * r][d]) = v;
