@@ -752,8 +752,10 @@ typedef struct {
  * own and theirs, and where it grew the earlier codes of the block (offsets below the first new
  * one) become rint(code * (old / new)). New codes are rint(x * (1 / scale)), ties to even;
  * non-finite elements count as 0, a scale below the smallest normal f32 is 0. The tokens of one
- * block must stand together in the call, in consecutive slots; one that leaves a gap is skipped
- * and reported (bit 2). */
+ * block must stand together in the call, in consecutive slots: one that leaves a gap, in slots or
+ * by skipped tokens before it, is skipped and reported (bit 2), as are those that follow it in the
+ * block. A block that comes up again after another block's tokens is not noticed; its codes and
+ * scales are then undefined. */
 int jkb_kv_append(jkb_kv_cache *cache, const jkb_rows *k, const jkb_rows *v,
                   const int32_t *slots, size_t n_tokens, void *stream);
 

@@ -1427,9 +1427,10 @@ class KvCache:
 def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, stream=None):
     """Quantizes the key and value rows [tokens, kv heads, head dim] (float32, float16 or
     bfloat16; parts of a fused projection may be strided) into their slots (int32; negative:
-    skipped). The tokens of a block stand together, in consecutive slots. A block's scale is its
-    absmax * float32(1 / 127): fresh where its first new token has offset 0, else the larger of its own and the
-    new rows', its earlier codes being rounded again where it grew."""
+    skipped). The tokens of a block stand together, in consecutive slots; one behind a gap or a
+    skipped token of its block is skipped too, and device_status reports it. A block's scale is its
+    absmax * float32(1 / 127): fresh where its first new token has offset 0, else the larger of its
+    own and the new rows', its earlier codes being rounded again where it grew."""
     kr = _rows(k, "k", cache.n_kv_heads, cache.head_dim)
     vr = _rows(v, "v", cache.n_kv_heads, cache.head_dim)
     n = slots.numel()
