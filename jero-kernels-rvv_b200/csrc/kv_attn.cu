@@ -852,17 +852,20 @@ template <class C>
 int launch_cfg(const AttnParams &p, int type, cudaStream_t st) {
     static_assert(dec_fits<C>(), "");
     static const char *fn = "attention_kv8";
-    const size_t smem = sizeof(DecSmem<C>) + 128 + 8 * ((size_t)p.n_seqs + 1);
-    static thread_local size_t allowed = 0;
+    constexpr size_t fixed = sizeof(DecSmem<C>) + 128;
+    constexpr size_t most = fixed + 8 * ((size_t)JKB_KV_MAX_SEQS + 1);
+    static_assert(most <= 227 * 1024, "shared memory");
+    const size_t smem = fixed + 8 * ((size_t)p.n_seqs + 1);
+    // The limit is one for all threads of the process: always the same value, so that no call
+    // lowers it under another.
     static thread_local int allowed_dev = -1;
     int dev = 0;
     cudaGetDevice(&dev);
-    if (dev != allowed_dev || smem > allowed) {
+    if (dev != allowed_dev) {
         cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<C>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)smem);
+                                             (int)most);
         if (e != cudaSuccess) return fail_cuda(e, fn);
-        allowed = smem;
         allowed_dev = dev;
     }
     cudaError_t e = launch_pdl(attn_decode_kernel<C>, dim3((unsigned)(num_sms() * DEC_CTAS)),
