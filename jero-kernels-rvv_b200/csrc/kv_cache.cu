@@ -882,9 +882,10 @@ int jkb_kv_build_tables(const jkb_kv_tables_args *a, void *stream) {
     for (const void *p : ptrs)
         if (int rc = check_align(p, 4, fn, "int32")) return rc;
     const size_t smem = (2 * a->n_seqs + 1) * 4;
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(
-            tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (smem > 48 * 1024) {  // always to the same value: it is one for all threads of the process
+        cudaError_t e = cudaFuncSetAttribute(tables_kernel,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (2 * JKB_KV_MAX_SEQS + 1) * 4);
         if (e != cudaSuccess) return fail_cuda(e, fn);
     }
     const size_t want = (a->n_slots + 4 * TABLE_THREADS - 1) / (4 * TABLE_THREADS);

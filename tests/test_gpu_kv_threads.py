@@ -44,3 +44,31 @@ def test_a_second_thread_with_fewer_sequences(jkb, dim, heads):
     kvref.check_attention(again, lse, ref, 40)
     kvref.check_attention(out, out_lse, [x[:few] for x in ref], 40)
     assert torch.equal(first, again)
+
+
+def test_tables_of_two_threads_at_once(jkb):
+    """More sequences than the default shared memory holds, of two sizes, in turn and at once."""
+
+    def call(n):
+        ctx, new = i32(np.zeros(n)), i32(np.ones(n))
+        table, slots, pos = i32(np.full((n, 1), -1)), i32(np.zeros(n)), i32(np.zeros(n))
+        starts, lens, counts = i32(np.zeros(n + 1)), i32(np.zeros(n)), i32(np.zeros(3))
+        st = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        free = i32(np.arange(n))
+        torch.cuda.synchronize()
+        for _ in range(200):
+            jkb.kv_build_tables(table, slots, pos, starts, lens, counts, ctx, new, free, 16,
+                                stream=st)
+        st.synchronize()
+        return counts.tolist()
+
+    assert call(8192) == [8192, 8192, 0]
+    results = {}
+    threads = [threading.Thread(target=lambda n=n: results.update({n: call(n)}))
+               for n in (8192, 6200)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert results == {n: [n, n, 0] for n in (8192, 6200)}
