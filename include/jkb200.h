@@ -770,7 +770,8 @@ int jkb_kv_append(jkb_kv_cache *cache, const jkb_rows *k, const jkb_rows *v,
  * negative, and from the last token on);
  * kv_lens [n_seqs], ctx + new (ctx where there was no room); counts [3]: new tokens, blocks
  * taken, sequences without room. Negative lengths count as 0. New tokens past n_slots get no
- * slot (counts[0] says how many there are). */
+ * slot (counts[0] says how many there are). An output that shares memory with an input or with
+ * another output is refused (JKB_E_BOUNDS): a step's kv_lens cannot be written over its ctx_lens. */
 #define JKB_KV_MAX_SEQS 8192
 typedef struct {
     int32_t *block_table;

@@ -680,6 +680,41 @@ int copy_launch(const jkb_kv_cache *c, const int32_t *blocks, size_t n, void *k,
     return e == cudaSuccess ? JKB_OK : fail_cuda(e, fn);
 }
 
+// Whether n ints at p share an element with `rows` rows of `width`, `stride` apart, at `table`.
+bool overlaps(const int32_t *table, size_t rows, size_t width, size_t stride, const int32_t *p,
+              size_t n) {
+    if (!rows || !width || !n) return false;
+    const uintptr_t a = (uintptr_t)table / 4, b = (uintptr_t)p / 4;
+    if (b < a) return n > a - b;
+    if (b - a >= (rows - 1) * stride + width) return false;
+    const size_t col = (b - a) % stride;
+    return col < width || n > stride - col;
+}
+
+// The kernel reads its inputs again after other CTAs have written their outputs, so no output may
+// share memory with an input or another output.
+int check_tables_apart(const jkb_kv_tables_args *a, const char *fn) {
+    const struct {
+        const int32_t *p;
+        size_t n;
+        const char *name;
+    } list[] = {{a->slots, a->n_slots, "slots"},         {a->positions, a->n_slots, "positions"},
+                {a->q_starts, a->n_seqs + 1, "q_starts"}, {a->kv_lens, a->n_seqs, "kv_lens"},
+                {a->counts, 3, "counts"},                 {a->ctx_lens, a->n_seqs, "ctx_lens"},
+                {a->new_lens, a->n_seqs, "new_lens"},     {a->free_blocks, a->n_free, "free_blocks"}};
+    constexpr int N = sizeof(list) / sizeof(list[0]), OUTPUTS = 5;
+    for (int i = 0; i < N; i++) {
+        if (overlaps(a->block_table, a->n_seqs, a->row_blocks, a->table_stride, list[i].p,
+                     list[i].n))
+            return fail(JKB_E_BOUNDS, fn, 0, 0, 0, "%s overlaps block_table", list[i].name);
+        for (int j = 0; j < i && j < OUTPUTS; j++)
+            if (overlaps(list[j].p, 1, list[j].n, list[j].n, list[i].p, list[i].n))
+                return fail(JKB_E_BOUNDS, fn, 0, 0, 0, "%s overlaps %s", list[i].name,
+                            list[j].name);
+    }
+    return JKB_OK;
+}
+
 int log2_block(size_t b) { return b == 16 ? 4 : b == 32 ? 5 : b == 64 ? 6 : b == 128 ? 7 : -1; }
 
 }  // namespace
@@ -881,6 +916,7 @@ int jkb_kv_build_tables(const jkb_kv_tables_args *a, void *stream) {
                           a->counts,      a->ctx_lens, a->new_lens,  a->free_blocks};
     for (const void *p : ptrs)
         if (int rc = check_align(p, 4, fn, "int32")) return rc;
+    if (int rc = check_tables_apart(a, fn)) return rc;
     const size_t smem = (2 * a->n_seqs + 1) * 4;
     if (smem > 48 * 1024) {  // always to the same value: it is one for all threads of the process
         cudaError_t e = cudaFuncSetAttribute(tables_kernel,

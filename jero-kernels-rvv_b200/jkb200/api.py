@@ -1447,7 +1447,8 @@ def kv_build_tables(block_table, slots, positions, q_starts, kv_lens, counts, ct
     new_lens[i]; the blocks it needs come from free_blocks, in order. Writes the rows' new
     entries, slots and positions of the new tokens (-1 where there was no room, and past the last
     token), q_starts [sequences + 1], kv_lens [sequences] and counts [3]: new tokens, blocks
-    taken, sequences without room."""
+    taken, sequences without room. No output may share memory with an input or another output
+    (kv_lens is not ctx_lens)."""
     ptr, n, width, stride = _table(block_table)
     n_slots = slots.numel()
     if (ctx_lens.numel() != n or new_lens.numel() != n or kv_lens.numel() != n
