@@ -786,7 +786,9 @@ typedef struct {
 int jkb_kv_build_tables(const jkb_kv_tables_args *args, void *stream);
 
 /* Scratch of the attention calls over caches of one head_dim: partial results where the tokens
- * of a sequence are split over the GPU. Calls that may overlap on the GPU need one each. */
+ * of a sequence are split over the GPU. Calls that may overlap on the GPU need one each. After a
+ * call whose wait expired (jkb_device_status, bit 3) its workspace is not used again, since pieces
+ * that did not arrive were not counted: destroy it and make another. */
 typedef struct jkb_attn_workspace jkb_attn_workspace;
 int jkb_attn_workspace_create(const jkb_kv_cache *cache, jkb_attn_workspace **out);
 int jkb_attn_workspace_destroy(jkb_attn_workspace *ws);

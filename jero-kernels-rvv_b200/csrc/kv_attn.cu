@@ -496,10 +496,11 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
 
         if (any) {
             const int st = s % STAGES;
-            if (!dead && !mbar_wait(&sm.full[warp][st], (phases >> st) & 1, &sm.abort_flag, p.err,
-                                    ERR_ATTN_WAIT))
-                dead = true;
-            phases ^= 1u << st;
+            // (each lane polls for itself; all go on, or none: what follows takes whole warps)
+            if (!dead)
+                dead = !__all_sync(~0u, mbar_wait(&sm.full[warp][st], (phases >> st) & 1,
+                                                  &sm.abort_flag, p.err, ERR_ATTN_WAIT));
+            if (!dead) phases ^= 1u << st;
         }
         if (any && !dead) {
             const uint8_t *stage = sm.ring[warp][s % STAGES];
@@ -661,7 +662,8 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
             }
         }
         __syncwarp();
-        if (s + STAGES < steps) issue(s + STAGES, next_src);
+        // (a barrier whose phase did not end must not be armed again)
+        if (s + STAGES < steps && !dead) issue(s + STAGES, next_src);
 
         if (!(flags & STEP_LAST)) continue;
         // ---- the piece ends: the warps' (m, l, o) into one ----
