@@ -1159,8 +1159,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
     }
 out:
-    // On expiry of a wait: the loads and MMAs in flight end (bounded) before the memory goes.
-    if (warp == 20 && lane == 0) {
+    // On expiry of a wait: the loads and MMAs in flight end (bounded) before the memory goes. (A
+    // commit follows its own thread's MMAs: the elected one's.)
+    __syncwarp();
+    if (warp == 20 && elect_one()) {
         tc_commit(&sm.done);
         const unsigned long long t0 = globaltimer();
         while (!mbar_try(&sm.done, 0) && globaltimer() - t0 < WAIT_NS) {
