@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
                 const bool on = tok < q.nq;
                 const int pos = q.len - q.nq + tok;
                 hi[r] = !on ? 0 : p.causal ? min(q.len, pos + 1) : q.len;
-                lo[r] = p.window ? max(0, pos - p.window + 1) : 0;
+                lo[r] = first_seen(p, pos);
                 m[r] = big[r] = -INFINITY;
                 l[r] = 0.0f;
 #pragma unroll
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(32 * NW, DEC_CTAS)
             const int pos_a = q.len - q.nq + tile * ROWS / p.group;
             const int pos_b = q.len - q.nq + last / p.group;
             all_hi = p.causal ? min(q.len, pos_a + 1) : q.len;
-            all_lo = p.window ? pos_b - p.window + 1 : 0;
+            all_lo = first_seen(p, pos_b);
         }
 
         if (any) {

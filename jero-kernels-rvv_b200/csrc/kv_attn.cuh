@@ -55,6 +55,12 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnParams &p, int i) {
     return s;
 }
 
+// The first token that a query at position pos sees (pos is negative for queries before the first
+// cached token; the difference is only taken where it cannot overflow).
+__device__ __forceinline__ int first_seen(const AttnParams &p, int pos) {
+    return p.window && pos >= p.window ? pos - p.window + 1 : 0;
+}
+
 // A bounded wait in few instructions (the roles' loops hold many): at most 2^20 tries of about a
 // microsecond.
 __device__ __forceinline__ bool mbar_wait_short(uint64_t *b, uint32_t parity,

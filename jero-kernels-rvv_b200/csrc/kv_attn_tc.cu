@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (lane == 0) mbar_arrive(&sm.q_empty);
             const int pos = cur.pos0 + (cur.row0 + row) / p.group;
             const int hi = p.causal ? min(cur.len, pos + 1) : cur.len;
-            const int lo = p.window ? max(0, pos - p.window + 1) : 0;
+            const int lo = first_seen(p, pos);
             const uint32_t end = it + cur.n;
             uint32_t i = it + ((it ^ wg) & 1);
             int key0 = cur.key0 + (int)(i - it) * TN;
@@ -1119,7 +1119,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         q.row0 = t.row0, q.head = head, q.q0 = s.q0, q.nq = s.nq;
                         q.pos0 = t.pos0, q.len = s.len, q.lo = t.lo, q.hi = t.hi;
                         q.all_hi = p.causal ? min(s.len, first + 1) : s.len;
-                        q.all_lo = p.window ? last - p.window + 1 : 0;
+                        q.all_lo = first_seen(p, last);
                         q.seq = seq;
                         q.cta0 = (int)(base / per);
                         q.cta1 = (int)((base + t.units - 1) / per);

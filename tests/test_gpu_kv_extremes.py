@@ -29,3 +29,15 @@ def test_queries_at_both_ends_of_the_range(jkb, kind, new, dim, q_exp, k_exp, sc
     ref = kvref.attention(c, q, table, lens, starts, scale, True, 0)
     kvref.check_attention(out, lse, ref, 300)
     assert jkb.device_status() == 0
+
+
+@pytest.mark.parametrize("window", [300, 301, 2**30, 2**31 - 200, 2**31 - 1, 2**31, 2**40])
+@pytest.mark.parametrize("lens,new", [([120], [3]), ([3], [5]), ([40], [200]), ([250, 90], [70, 130])])
+def test_windows_beyond_every_context(jkb, window, lens, new):
+    """As no window, for queries before the first cached token too (more new tokens than cached
+    ones): without a causal mask they see every token."""
+    c, cache, q, table, starts = setup(jkb, lens, new, 4, 2, 64, 16, "f32", seed=5)
+    for causal in (True, False):
+        out, lse = run(jkb, cache, q, table, lens, starts, 0.1, causal, window)
+        ref = kvref.attention(c, q, table, lens, starts, 0.1, causal, 0)
+        kvref.check_attention(out, lse, ref, max(lens))
