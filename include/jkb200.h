@@ -766,8 +766,8 @@ int jkb_kv_append(jkb_kv_cache *cache, const jkb_rows *k, const jkb_rows *v,
  * tokens exceed its row takes none; neither does one for which the list has not enough left, nor
  * any later one that needs a block. Outputs, all device int32: q_starts [n_seqs + 1], the
  * exclusive sums of new_lens; slots and positions [n_slots], for the new tokens of all sequences
- * in order (-1 for the tokens of a sequence that found no room, or whose held block's entry is
- * negative, and from the last token on);
+ * in order (-1 for the tokens of a sequence that found no room, or whose block's id is negative or,
+ * which is reported as bit 2, too large for a slot of 32 bits, and from the last token on);
  * kv_lens [n_seqs], ctx + new (ctx where there was no room); counts [3]: new tokens, blocks
  * taken, sequences without room. Negative lengths count as 0. New tokens past n_slots get no
  * slot (counts[0] says how many there are). An output that shares memory with an input or with

@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(TABLE_THREADS)
                   int32_t *__restrict__ q_starts, int32_t *__restrict__ kv_lens,
                   int32_t *__restrict__ counts, const int32_t *__restrict__ ctx_lens,
                   const int32_t *__restrict__ new_lens, const int32_t *__restrict__ free_blocks,
-                  int n_free, int log_block) {
+                  int n_free, int log_block, int *err) {
     extern __shared__ int32_t table_smem[];
     int32_t *start = table_smem;             // [n_seqs + 1], clamped to INT_MAX
     int32_t *base = table_smem + n_seqs + 1; // [n_seqs] first free-list index; -1: no room
@@ -147,6 +147,10 @@ __global__ void __launch_bounds__(TABLE_THREADS)
             const int id = j < first ? table[(size_t)s * table_stride + j]
                                      : __ldg(free_blocks + base[s] + j - first);
             if (id < 0) continue;
+            if (id > INT32_MAX >> log_block) {  // its slots would not fit 32 bits
+                atomicOr(err, ERR_KV_RANGE);
+                continue;
+            }
             sl[k] = (id << log_block) + (p & mask);
             po[k] = p;
         }
@@ -927,11 +931,13 @@ int jkb_kv_build_tables(const jkb_kv_tables_args *a, void *stream) {
     const size_t want = (a->n_slots + 4 * TABLE_THREADS - 1) / (4 * TABLE_THREADS);
     const size_t most = 2 * (size_t)num_sms();
     const unsigned grid = (unsigned)(want < 1 ? 1 : want > most ? most : want);
+    int *err = device_error_word();
+    if (!err) return fail(JKB_E_CUDA, fn, 0, 0, 0, "no device error word");
     cudaError_t e = launch_pdl(tables_kernel, dim3(grid), dim3(TABLE_THREADS), smem,
                                as_stream(stream), a->block_table, (int)a->n_seqs,
                                (int)a->row_blocks, a->table_stride, a->slots, a->positions,
                                (int)a->n_slots, a->q_starts, a->kv_lens, a->counts, a->ctx_lens,
-                               a->new_lens, a->free_blocks, (int)a->n_free, lb);
+                               a->new_lens, a->free_blocks, (int)a->n_free, lb, err);
     return e == cudaSuccess ? JKB_OK : fail_cuda(e, fn);
 }
 
