@@ -1506,7 +1506,7 @@ def attention_kv8(out, q, cache: KvCache, workspace: AttentionWorkspace, block_t
         raise ValueError(f"{out.shape[0]} output rows for {n} queries")
     if window < 0 or max_new < 0:
         raise ValueError("window and max_new cannot be negative")
-    if lse is not None and (lse.dtype != torch.float32 or lse.numel() != n * heads):
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (n, heads)):
         raise ValueError(f"lse: expected float32 [{n}, {heads}]")
     ptr, seqs, width, stride = _table(block_table)
     if kv_lens.numel() != seqs or q_starts.numel() != seqs + 1:
