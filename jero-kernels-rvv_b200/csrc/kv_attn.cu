@@ -977,8 +977,9 @@ int jkb_attention_kv8(const jkb_attn_args *a, void *stream) {
     if (a->n_seqs > JKB_KV_MAX_SEQS)
         return fail(JKB_E_BOUNDS, fn, 0, a->n_seqs, JKB_KV_MAX_SEQS, "%zu sequences, at most %d",
                     a->n_seqs, JKB_KV_MAX_SEQS);
-    if (a->n_tokens > (size_t)INT32_MAX / a->n_heads)
-        return fail(JKB_E_BOUNDS, fn, 0, a->n_tokens, (size_t)INT32_MAX / a->n_heads,
+    // (a tile's row numbers go up to 127 beyond the last)
+    if (a->n_tokens > (size_t)(INT32_MAX - 128) / a->n_heads)
+        return fail(JKB_E_BOUNDS, fn, 0, a->n_tokens, (size_t)(INT32_MAX - 128) / a->n_heads,
                     "%zu query tokens of %zu heads in one call", a->n_tokens, a->n_heads);
     if (a->row_blocks > (size_t)INT32_MAX / c->block_tokens || a->table_stride < a->row_blocks)
         return fail(JKB_E_BOUNDS, fn, 0, a->row_blocks, a->table_stride,

@@ -23,3 +23,12 @@ def test_lse_of_another_shape(jkb):
             call(jkb, q, out, lse)
     q = q[:0]
     call(jkb, q, out[:0], torch.empty(0, 4, device="cuda"), (0, 0))
+
+
+@pytest.mark.parametrize("heads", [1, 3])
+def test_more_query_rows_than_row_numbers(jkb, heads):
+    """Broadcast rows, of which there is one in memory: refused before anything runs."""
+    n = 2**31 // heads - 100 // heads
+    q = torch.zeros(1, heads, 8, device="cuda").expand(n, heads, 8)
+    with pytest.raises(jkb.TensorBoundsError):
+        call(jkb, q, torch.zeros(1, heads, 8, device="cuda").expand(n, heads, 8), starts=(0, n))
