@@ -68,3 +68,28 @@ def test_lse_of_every_row_type(jkb, kind, lens, new, heads, dim):
     c, _, q, table, starts = setup(jkb, lens, new, heads, 2, dim, 32, kind, seed=dim)
     check(jkb, c, q, table, lens, starts, dim ** -0.5)
     check(jkb, c, q, table, lens, starts, dim ** -0.5, causal=False, window=77)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(64, 8, 128), (96, 8, 96), (64, 32, 64), (32, 2, 128),
+                                                (24, 8, 256)])
+def test_few_row_scores_in_24_bits(jkb, kind, heads, kv_heads, dim):
+    """With one cached token lse is the score itself. An element of q is off by half a unit of its
+    row's 24 bits (the largest over 8355700, so 1.01 2^-24 of it) and by 2^-24 of itself; f32 steps
+    (the unit and its inverse, the scales, the sum of the digits' products) by 2^-20 of the score;
+    its weight, the logarithm and their sum by 2^-20. Digits of 16 bits would be 16 times that off or
+    more (the same inputs rounded to 16 bits in numpy)."""
+    for seed in range(4):
+        lens = [1] * 6
+        c, cache, q, table, starts = setup(jkb, lens, lens, heads, kv_heads, dim, 16, kind, seed=seed)
+        scale = dim ** -0.5
+        _, lse = run(jkb, cache, q, table, lens, starts, scale)
+        k = torch.from_numpy(c.k[table[:, 0], :, 0]).cuda().double()
+        k = k * torch.from_numpy(c.ks[table[:, 0]]).cuda().double()[..., None]
+        k = k.repeat_interleave(heads // kv_heads, 1)
+        x = q.double()
+        s = scale * (x * k).sum(2)
+        tol = scale * 2.0 ** -24 * (1.01 * x.abs().amax(2) * k.abs().sum(2) + (x * k).abs().sum(2))
+        tol = tol + 2.0 ** -20 * (s.abs() + 1)
+        err = (lse.double() - s).abs()
+        assert bool((err <= tol).all()), float((err / tol).max())
