@@ -33,11 +33,11 @@
 // which one that is.
 //
 // Measured, 8 kv heads of 128 dims: 64 sequences of 500 to 9000 tokens (32 query heads, f32, 0.59
-// GB of codes) take 134 us, 4.4 TB/s of codes; one of 131,071 tokens (64 query heads, bf16, 0.27
-// GB) 65 us; one of 700 tokens (32, f32) 11 us. Long contexts are bound by the issue of the 744
-// instructions a step, of which two warps a sub-partition issue 0.4 a clock (the copies alone
-// take 105 us of the 134), by the slowest SMs (12 us after the median) and the joins (4 us);
-// short row tiles by their own start (q to digits, 1.5 us) and end (1.5 us): 5 us one of a step.
+// GB of codes) take 128 to 133 us, 4.4 to 4.6 TB/s of codes; one of 131,071 tokens (64 query heads,
+// bf16, 0.27 GB) 64.5 us; one of 700 tokens (32, f32) 10 us. Long contexts are bound by the latency
+// of a step's 736 instructions, which depend on one another and of which two warps a sub-partition
+// issue 0.42 a clock (1.8 of an instruction's 4.2 clocks wait for the one before), short row tiles
+// also by their starts and ends, where the warps meet at barriers.
 #include "kv_attn.cuh"
 #include "ptx.cuh"
 

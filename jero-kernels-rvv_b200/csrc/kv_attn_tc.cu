@@ -19,7 +19,8 @@
 // Work: MMA time is (DIM / 16) NQ + 8 NP steps a unit against 16 for one plain product pair; the
 // exponentials are 128 x 128 a unit on 16 lanes an SM and clock, about as long as two products;
 // and the issue slots: about 850 (16-bit rows) to 1200 (f32) a softmax warp, 500 a conversion
-// warp and 200 an accumulation warp a unit, on each of the SM's four sub-partitions.
+// warp and 200 an accumulation warp a unit, on each of the SM's four sub-partitions (2250 to 2750 in
+// all with the tiles' starts and ends).
 // One CTA an SM, six warpgroups, every hand-over an mbarrier:
 //   0, 1  the query rows of a new tile; softmax, every other unit each (a unit's needs nothing of
 //         the one before): a thread a row; S from TMEM, p's parts back over it
@@ -43,12 +44,12 @@
 // kv_attn.cu).
 //
 // Measured, 32 query heads over 8 kv heads of 128 dims: a causal prompt of 2048 f32 tokens behind
-// 1111 cached ones takes 213 us (337 TFLOP/s of its two products; the 5 f16 products that f32
-// needs run at 840), one of 8192 bf16 tokens 997 us (551 TFLOP/s; with p's second part 827; 904
-// us before the power limit lowers the clock); nine ragged f16 chunks, 5331 tokens of 14 query
+// 1111 cached ones takes 212 us (337 TFLOP/s of its two products; the 5 f16 products that f32
+// needs run at 840), one of 8192 bf16 tokens 1000 us (550 TFLOP/s; with p's second part 825); nine ragged f16 chunks, 5331 tokens of 14 query
 // heads over 2 of 80 dims, 166 us (155 with p in one f16 part, 11 bits, whose error is as large as
-// the output's rounding). What bounds a unit are the issue slots above; a tile's start
-// and end cost as much as 5 units.
+// the output's rounding). A unit takes 3400 (16-bit rows) to 4600 clocks (f32), of which the issue
+// slots fill 62 and 47 % and the MMAs 42 and 43 %: what bounds it is the latency of the roles' waits
+// for tensor memory and for one another. A tile's start and end cost as much as 5 units.
 #include "kv_attn.cuh"
 #include "ptx.cuh"
 

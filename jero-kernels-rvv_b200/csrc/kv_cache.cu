@@ -25,8 +25,9 @@ constexpr int TABLE_THREADS = 512;
 // over at most JKB_KV_MAX_SEQS entries, read from L2), which is cheaper than a second launch or a
 // wait between CTAs; it then writes its share of the rows, lengths and slots. A new token's
 // block is looked up in the free list rather than in the row that some other CTA is writing.
-// 8 bytes a token move; below about 100,000 tokens the launch and the scan's latency bound it:
-// 4.4 us for 24 sequences of one token, 4.8 us for 1500 of 350 on average.
+// 8 bytes a token move. The launch and the scans' latency bound a decode step (24 sequences of one
+// token: 4.3 us), the search of each four tokens' sequence a large one (1500 of 350 tokens on
+// average: 10.2 us, 60 % of the issue slots).
 __global__ void __launch_bounds__(TABLE_THREADS)
     tables_kernel(int32_t *__restrict__ table, int n_seqs, int row_blocks, size_t table_stride,
                   int32_t *__restrict__ slots, int32_t *__restrict__ positions, int n_slots,
@@ -232,10 +233,11 @@ struct Run {
 // A first pass takes the rows' absmax; the second reads them again (from L1 or L2: a block's rows
 // are at most 64 KB) and writes 16 bytes of codes at a time: a key patch is 16 dims of one token,
 // a value patch 4 dims of 4 tokens. Old bytes are read only where a patch keeps some of them.
-// Instructions bound it, their number an element and, as each runs a few times a run, their
-// fetching: the rare paths are loops over little code. (Patches kept in registers between the
-// passes, in eight times the code, took twice as long.) 5985 f32 tokens of 8 heads of 128 take 23
-// us (2.6 TB/s of rows and codes), 16,411 bf16 tokens 40 us (2.5 TB/s), 24 single tokens 8 us.
+// Instructions bound it, 29 an element (f32) or 25 (bf16), which fill 57 to 66 % of the issue slots,
+// the waits between the two passes and, as each instruction runs a few times a run, their fetching:
+// the rare paths are loops over little code. (Patches kept in registers between the passes, in eight
+// times the code, took twice as long.) 5985 f32 tokens of 8 heads of 128 take 22 us (2.8 TB/s of rows
+// and codes), 16,411 bf16 tokens 41 us (2.5 TB/s), 24 single tokens 5 us.
 template <int TYPE, bool VEC>
 __device__ __forceinline__ void append_run(const Run &r, const AppendSide &src, bool value,
                                            int head, int tid, int team, uint8_t *codes,
@@ -549,7 +551,7 @@ enum { COPY_IMPORT, COPY_EXPORT, COPY_READ };
 
 // One thread a 16-byte patch of codes (a key patch: 16 dims of a token; a value patch: 4 dims of
 // 4 tokens). MODE COPY_READ writes 64 bytes of f32 values for it, which bounds the kernel: 257
-// blocks of 64 tokens and 8 heads of 128 dims take 33 us, 5.1 TB/s.
+// blocks of 64 tokens and 8 heads of 128 dims take 34 us, 5.0 TB/s.
 template <int MODE, int DP>
 __global__ void __launch_bounds__(COPY_THREADS)
     copy_kernel(const int32_t *__restrict__ blocks, uint8_t *__restrict__ codes,
