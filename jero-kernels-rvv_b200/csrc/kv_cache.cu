@@ -486,17 +486,18 @@ __global__ void __launch_bounds__(APPEND_THREADS)
     // A run starts at a token whose block is not that of the last token before it, skipped ones
     // aside: two runs of one block would rewrite its scale and codes at the same time.
     if (warp < 2) {
-        const unsigned there0 = __ballot_sync(~0u, lane < span && s_slot[1 + lane] >= 0);
-        const unsigned there1 = __ballot_sync(~0u, 32 + lane < span && s_slot[33 + lane] >= 0);
-        const unsigned long long earlier =
-            (there0 | (unsigned long long)there1 << 32) & ((1ull << tid) - 1);
         const int s = tid < span ? s_slot[1 + tid] : -1;
-        int before = earlier ? s_slot[64 - __clzll(earlier)] : s_slot[0];
-        const bool far = s >= 0 && !earlier && before < 0;  // (the range's first, if any)
-        if (__any_sync(~0u, far)) {
+        int before = s_slot[tid];
+        if (__any_sync(~0u, s >= 0 && before < 0)) {
+            const unsigned there0 = __ballot_sync(~0u, lane < span && s_slot[1 + lane] >= 0);
+            const unsigned there1 = __ballot_sync(~0u, 32 + lane < span && s_slot[33 + lane] >= 0);
+            const unsigned long long earlier =
+                (there0 | (unsigned long long)there1 << 32) & ((1ull << tid) - 1);
+            before = earlier ? s_slot[64 - __clzll(earlier)] : s_slot[0];
+            const bool far = s >= 0 && !earlier && before < 0;  // (the range's first, if any)
             int last = -1;
 #pragma unroll 1
-            for (int end = first - 2; end >= 0 && last < 0; end -= 32) {
+            for (int end = __any_sync(~0u, far) ? first - 2 : -1; end >= 0 && last < 0; end -= 32) {
                 int x = end >= lane ? __ldg(slots + (end - lane)) : -1;
                 if (x >= n_slots) x = -1;
                 const unsigned there = __ballot_sync(~0u, x >= 0);
